@@ -336,6 +336,120 @@ OMOE_API int omoe_route_noalloc(const void *x_dev, const float *w_router_dev, co
                                 float *topk_w_dev, int32_t *counts_dev, void *cuda_stream);
 OMOE_API const char *omoe_route_noalloc_error(void);
 
+/*
+ * Operators for hosts that run the parts around this layer, or experts of their own, themselves.  They take no
+ * handle and keep nothing between calls: every buffer, workspaces included, is the caller's DEVICE memory, so
+ * calls on different streams, and captured graphs, do not share anything unless the caller makes them.  They
+ * enqueue kernels on the given stream, never synchronise the host and never allocate; the same inputs give the
+ * same bits.  Results are undefined where an output overlaps an input or another output, unless stated;
+ * such calls are refused where the library can see it.  Error text: omoe_ops_error(), per host thread, valid until the
+ * thread's next call of one of these entry points.
+ *
+ * Rows are row-major with a leading dimension (elements from one row to the next, at least d).  Any width,
+ * leading dimension and element-aligned address is taken; rows whose width is a multiple of 8 and whose address
+ * and leading dimension keep every row 16-byte aligned move as vectors, others element by element.
+ */
+OMOE_API const char *omoe_ops_error(void);
+
+/*
+ * Token rows sorted by expert and back.
+ *
+ * A plan says where every pick's row lies.  The caller fills in the sizes and its device buffers, and
+ * omoe_sort_plan writes the buffers from the picks topk_idx [T, top_k] (as omoe_route_noalloc leaves them):
+ *   counts [E]     picks of each expert;
+ *   offsets [E+1]  first row of each expert: offsets[e+1] = offsets[e] + counts[e] rounded up to row_align;
+ *   pos [T*top_k]  row of each pick: an expert's picks lie in the order of the flat pick index t*top_k + j;
+ *   perm [rows_cap] the flat pick index of each row, -1 for padding rows and for the rows from offsets[E] on.
+ * A pick outside [0, E) (a token of a padded batch, a pick over an expert's capacity) has no row: pos = -1.  The
+ * same expert may be picked twice by a token.  rows_cap must be at least omoe_sort_rows_cap(...), which returns
+ * T*top_k plus the padding that the experts with picks can need, or a negative status.
+ * Limits: n_experts <= OMOE_SORT_MAX_EXPERTS, top_k <= 16, rows_cap <= 0x7fff0000; leading dimensions
+ * of all the operators: at most 2^30.
+ *
+ * With N picks that have a row:
+ *   omoe_sort_rows            xs[pos[t,j], :] = x[t, :] for every pick; padding rows (inside [0, offsets[E])) are
+ *                             written as zeros, so that products over whole segments stay finite; rows from
+ *                             offsets[E] on are left as they were.
+ *   omoe_sort_rows_backward   dx[t, :] = sum over the token's picks of dxs[pos[t,j], :].
+ *   omoe_unsort_rows          y[t, :] = sum over the token's picks, in pick order, of w[t,j] * ys[pos[t,j], :].
+ *   omoe_unsort_rows_backward dys[pos[t,j], :] = w[t,j] * dy[t, :], padding rows zero, later rows as they were;
+ *                             dw[t,j] = <dy[t, :], ys[pos[t,j], :]>, 0 for picks without a row.
+ * w and dw are [T, top_k] fp32; w = NULL stands for weights of 1, dw = NULL leaves the weights' gradient out (ys may then be
+ * NULL too).  Sums are fp32, rounded once; a token without any pick gets zeros.  Each matrix has its own element type; dys has
+ * that of ys.  Nothing is read from padding rows or from the rows behind them.
+ */
+#define OMOE_SORT_MAX_EXPERTS 1024
+typedef struct omoe_sort {
+    int32_t n_tokens, top_k, n_experts;
+    int32_t row_align;  /* >= 1; 128 gives every expert whole tensor-core tiles */
+    int64_t rows_cap;   /* rows of the sorted buffers, entries of perm */
+    int32_t *pos, *perm, *counts, *offsets; /* device */
+} omoe_sort;
+
+OMOE_API int64_t omoe_sort_rows_cap(int32_t n_tokens, int32_t top_k, int32_t n_experts, int32_t row_align);
+OMOE_API int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cuda_stream);
+OMOE_API int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_t x_dtype, void *xs_dev,
+                            int64_t ldxs, int32_t xs_dtype, int32_t d, void *cuda_stream);
+OMOE_API int omoe_sort_rows_backward(const omoe_sort *plan, const void *dxs_dev, int64_t lddxs, int32_t dxs_dtype,
+                                     void *dx_dev, int64_t lddx, int32_t dx_dtype, int32_t d, void *cuda_stream);
+OMOE_API int omoe_unsort_rows(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32_t ys_dtype,
+                              const float *w_dev, void *y_dev, int64_t ldy, int32_t y_dtype, int32_t d,
+                              void *cuda_stream);
+OMOE_API int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t lddy, int32_t dy_dtype,
+                                       const void *ys_dev, int64_t ldys, int32_t ys_dtype, const float *w_dev,
+                                       void *dys_dev, int64_t lddys, float *dw_dev, int32_t d, void *cuda_stream);
+
+/*
+ * Layer norm of T rows of width d: y = (x - mean) * rstd * gamma + beta, mean and rstd = 1/sqrt(var + eps) per
+ * row, var the mean of the squared differences (taken after the mean, in fp32).  The norm in front of the layer for blocks
+ * that are not built on the RMSNorm of omoe_forward_block.  gamma and beta are fp32 [d]; NULL stands for 1 and 0.
+ * mean and rstd [T] fp32 are written unless NULL; the backward pass takes them.
+ *
+ * omoe_layer_norm_backward: with g = dy * gamma and h = (x - mean) * rstd,
+ *   dx = rstd * (g - mean(g) - h * mean(g * h)) of x's element type, dgamma = sum over the rows of dy * h,
+ *   dbeta = sum over the rows of dy, fp32, overwritten.  dgamma and dbeta may be NULL.  workspace_dev holds at least
+ * omoe_layer_norm_backward_workspace(T, d) bytes, 16-byte aligned, whose contents do not matter.
+ */
+OMOE_API int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float *gamma_dev,
+                             const float *beta_dev, float eps, void *y_dev, int64_t ldy, int32_t y_dtype,
+                             float *mean_dev, float *rstd_dev, int32_t T, int32_t d, void *cuda_stream);
+OMOE_API int64_t omoe_layer_norm_backward_workspace(int32_t T, int32_t d);
+OMOE_API int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype, const void *x_dev, int64_t ldx,
+                                      int32_t x_dtype, const float *gamma_dev, const float *mean_dev,
+                                      const float *rstd_dev, void *dx_dev, int64_t lddx, float *dgamma_dev,
+                                      float *dbeta_dev, int32_t T, int32_t d, void *workspace_dev,
+                                      int64_t workspace_bytes, void *cuda_stream);
+
+/*
+ * Gradient norm over many tensors, and clipping: what an engine does between back() and update() with the
+ * gradients omoe_get_weight_grads left in its tensors and all the others.  `grads` and `out` are HOST arrays (read
+ * before the call returns) of contiguous DEVICE tensors; any count from 0 and any element-aligned address.
+ *
+ *   omoe_grad_norm   *norm_dev = sqrt(sum of the squares of all elements), fp32.  The squares are summed so that they
+ *                    neither overflow nor vanish for any finite fp32 gradients.
+ *   omoe_grad_scale  out = c * grads with c = min(1, max_norm / (*norm_dev + 1e-6)), rounded once.  Ranks that hold
+ *                    different gradients (expert parallelism) sum the squares of their norms between the two calls.
+ *   omoe_grad_clip   both, with fewer launches.
+ *
+ * out = NULL scales in place (nothing is written when c = 1).  Otherwise out[i] has grads[i]'s count and dtype.  The tensors
+ * of the list must not overlap; out[i] may be grads[i] itself.  Where the norm is not finite c is 1: the gradients arrive as they
+ * are, and the caller sees the norm.  max_norm >= 0, infinity included.  workspace_dev holds OMOE_GRAD_WORKSPACE_BYTES,
+ * 16-byte aligned, whose contents do not matter.
+ */
+typedef struct omoe_tensor {
+    void *ptr;      /* device */
+    int64_t count;  /* elements */
+    int32_t dtype;  /* OMOE_F32 or OMOE_BF16 */
+    int32_t reserved;
+} omoe_tensor;
+#define OMOE_GRAD_WORKSPACE_BYTES 16384
+OMOE_API int omoe_grad_norm(const omoe_tensor *grads, int32_t n, float *norm_dev, void *workspace_dev,
+                            int64_t workspace_bytes, void *cuda_stream);
+OMOE_API int omoe_grad_scale(const omoe_tensor *grads, const omoe_tensor *out, int32_t n, const float *norm_dev,
+                             float max_norm, void *cuda_stream);
+OMOE_API int omoe_grad_clip(const omoe_tensor *grads, const omoe_tensor *out, int32_t n, float max_norm,
+                            float *norm_dev, void *workspace_dev, int64_t workspace_bytes, void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,4 +13,8 @@ def __getattr__(name):
         from . import layer
 
         return getattr(layer, name)
+    if name in ("TokenSort", "layer_norm", "layer_norm_backward", "LNLayer", "GradList"):
+        from . import ops
+
+        return getattr(ops, name)
     raise AttributeError(name)

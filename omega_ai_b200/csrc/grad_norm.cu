@@ -1,0 +1,358 @@
+// The global norm of many gradient tensors, and clipping by it.
+//
+// All tensors together are one sequence of chunks of kChunkElems elements (a tensor's last one may be shorter); every block
+// takes an equal, contiguous part of it.  The table of tensors travels as a kernel parameter, so a call needs no copy
+// and a captured graph keeps its own.
+#include "ops.cuh"
+
+#include <float.h>
+#include <math.h>
+#include <stdlib.h>
+
+namespace omoe {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPerThread = 16;
+constexpr int kChunkElems = kThreads * kPerThread;
+constexpr int kSlots = OMOE_GRAD_WORKSPACE_BYTES / 8;  // blocks' sums in the workspace
+
+struct Entry {
+    const void *in;
+    void *out;
+    int64_t count;
+    int32_t first;  // chunk
+    int32_t dtype;
+};
+// As many tensors as one launch takes: few, or what fits the kernel parameters.
+template <int N>
+struct Table {
+    Entry e[N];
+    int32_t n, chunks;
+};
+constexpr int kFew = 48, kMany = 1000;
+
+// Squares of up to kPerThread values.  In fp32 first, with four chains; where that overflows, or is so small that squares
+// have lost digits, again in fp64 (the squares of fp32 values are exact there and their sum stays in range).
+__device__ __forceinline__ double squares(const float (&v)[kPerThread]) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kPerThread; i++) s[i & 3] = fmaf(v[i], v[i], s[i & 3]);
+    const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+    if (sum > 1e-20f && sum < 1e37f) return (double)sum;
+    double d = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerThread; i++) d = fma((double)v[i], (double)v[i], d);
+    return d;
+}
+
+__device__ __forceinline__ double block_sum(double v, double *s) {
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double sum = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); i++) sum += s[i];
+    __syncthreads();
+    return sum;
+}
+
+// The values of this thread in the chunk that starts at `p` with n elements; missing ones are 0.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T *p, int n, float (&v)[kPerThread]) {
+    constexpr int V = 16 / sizeof(T);
+    if (n == kChunkElems && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        uint4 r[kPerThread / V];
+#pragma unroll
+        for (int i = 0; i < kPerThread / V; i++) r[i] = *(reinterpret_cast<const uint4 *>(p) + i * kThreads + threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < kPerThread / V; i++) {
+            const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (V == 4) v[i * 4 + j] = __uint_as_float(w[j]);
+                else {
+                    v[i * 8 + 2 * j] = __uint_as_float(w[j] << 16);
+                    v[i * 8 + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPerThread; i++) {
+            const int at = i * kThreads + threadIdx.x;
+            v[i] = at < n ? (float)p[at] : 0.f;
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const T *p, T *o, int n, float c) {
+    constexpr int V = 16 / sizeof(T);
+    if (n == kChunkElems && ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15u) == 0) {
+        float v[kPerThread];
+        load_chunk(p, n, v);
+#pragma unroll
+        for (int i = 0; i < kPerThread / V; i++) {
+            uint4 r;
+            if constexpr (V == 4)
+                r = make_uint4(__float_as_uint(v[i * 4] * c), __float_as_uint(v[i * 4 + 1] * c), __float_as_uint(v[i * 4 + 2] * c),
+                               __float_as_uint(v[i * 4 + 3] * c));
+            else
+                r = make_uint4(pack_bf16(v[i * 8] * c, v[i * 8 + 1] * c), pack_bf16(v[i * 8 + 2] * c, v[i * 8 + 3] * c),
+                               pack_bf16(v[i * 8 + 4] * c, v[i * 8 + 5] * c), pack_bf16(v[i * 8 + 6] * c, v[i * 8 + 7] * c));
+            *(reinterpret_cast<uint4 *>(o) + i * kThreads + threadIdx.x) = r;
+        }
+    } else {
+        for (int at = threadIdx.x; at < n; at += kThreads) o[at] = (T)((float)p[at] * c);
+    }
+}
+
+// Calls f(entry, first element, elements) for every chunk of this block's part.
+template <int N, typename F>
+__device__ __forceinline__ void walk(const Table<N> &t, F f) {
+    const int lo = (int)((int64_t)t.chunks * blockIdx.x / gridDim.x), hi = (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x);
+    if (lo >= hi) return;
+    int i = 0;
+    for (int a = 0, b = t.n; a + 1 < b;) {  // the last tensor that starts at or before lo
+        const int mid = (a + b) >> 1;
+        if (t.e[mid].first <= lo) a = mid;
+        else b = mid;
+        i = a;
+    }
+    for (int c = lo; c < hi; c++) {
+        while (i + 1 < t.n && t.e[i + 1].first <= c) i++;
+        const Entry &e = t.e[i];
+        const int64_t at = (int64_t)(c - e.first) * kChunkElems;
+        f(e, at, (int)min((int64_t)kChunkElems, e.count - at));
+    }
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads)
+grad_squares_kernel(const __grid_constant__ Table<N> t, double *__restrict__ slots, int add) {
+    __shared__ double s[kThreads / 32];
+    pdl_trigger();
+    pdl_wait();
+    double sum = 0.0;
+    walk(t, [&](const Entry &e, int64_t at, int n) {
+        float v[kPerThread];
+        if (e.dtype == OMOE_F32) load_chunk(static_cast<const float *>(e.in) + at, n, v);
+        else load_chunk(static_cast<const __nv_bfloat16 *>(e.in) + at, n, v);
+        sum += squares(v);
+    });
+    sum = block_sum(sum, s);
+    if (threadIdx.x == 0) slots[blockIdx.x] = add ? slots[blockIdx.x] + sum : sum;
+}
+
+__device__ __forceinline__ float norm_of(const double *slots, int n, double *s) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) sum += slots[i];
+    return (float)sqrt(block_sum(sum, s));
+}
+
+__global__ void __launch_bounds__(kThreads)
+grad_norm_kernel(const double *__restrict__ slots, int n, float *__restrict__ norm) {
+    __shared__ double s[kThreads / 32];
+    pdl_trigger();
+    pdl_wait();
+    const float v = norm_of(slots, n, s);
+    if (threadIdx.x == 0) *norm = v;
+}
+
+// c = min(1, max_norm / (norm + 1e-6)); 1 where the norm is not finite.  Every block works it out, from the sums of the blocks
+// that squared (slots) or from the norm handed over.
+template <int N>
+__global__ void __launch_bounds__(kThreads)
+grad_scale_kernel(const __grid_constant__ Table<N> t, const double *__restrict__ slots, int n_slots, const float *norm_in,
+                  float *norm_out, float max_norm, int in_place) {
+    __shared__ double s[kThreads / 32];
+    pdl_trigger();
+    pdl_wait();
+    const float norm = slots ? norm_of(slots, n_slots, s) : *norm_in;
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+    float c = 1.f;
+    if (norm < INFINITY) c = (float)fmin(1.0, (double)max_norm / ((double)norm + 1e-6));
+    if (in_place && c == 1.f) return;
+    walk(t, [&](const Entry &e, int64_t at, int n) {
+        if (e.dtype == OMOE_F32) scale_chunk(static_cast<const float *>(e.in) + at, static_cast<float *>(e.out) + at, n, c);
+        else
+            scale_chunk(static_cast<const __nv_bfloat16 *>(e.in) + at, static_cast<__nv_bfloat16 *>(e.out) + at, n, c);
+    });
+}
+
+struct Span {
+    uintptr_t lo, hi;
+    int32_t i;
+};
+int by_address(const void *a, const void *b) {
+    const Span *x = static_cast<const Span *>(a), *y = static_cast<const Span *>(b);
+    return x->lo < y->lo ? -1 : x->lo > y->lo;
+}
+
+// The spans of a list by address, empty tensors left out; returns how many.
+int spans_of(const omoe_tensor *t, int n, Span *s) {
+    int m = 0;
+    bool sorted = true;
+    for (int i = 0; i < n; i++) {
+        if (t[i].count == 0) continue;
+        s[m].lo = reinterpret_cast<uintptr_t>(t[i].ptr);
+        s[m].hi = s[m].lo + (uintptr_t)t[i].count * (t[i].dtype == OMOE_BF16 ? 2 : 4);
+        s[m].i = i;
+        sorted = sorted && (m == 0 || s[m - 1].lo <= s[m].lo);
+        m++;
+    }
+    if (!sorted) qsort(s, m, sizeof(Span), by_address);
+    return m;
+}
+
+int check_list(const omoe_tensor *grads, const omoe_tensor *out, int n, bool writes, const char *fn) {
+    if (n < 0 || (n > 0 && !grads)) return ops_fail(OMOE_ERR_INVALID, fn, "bad list of tensors");
+    for (int i = 0; i < n; i++) {
+        const omoe_tensor &g = grads[i];
+        if (g.dtype != OMOE_F32 && g.dtype != OMOE_BF16) return ops_fail(OMOE_ERR_INVALID, fn, "a dtype is neither OMOE_F32 nor OMOE_BF16");
+        if (g.count < 0 || g.count > ((int64_t)1 << 42)) return ops_fail(OMOE_ERR_INVALID, fn, "a tensor's count is out of range");
+        if (g.count > 0 && !g.ptr) return ops_fail(OMOE_ERR_INVALID, fn, "null tensor");
+        const uintptr_t elem = g.dtype == OMOE_BF16 ? 2 : 4;
+        if (misaligned(g.ptr, elem)) return ops_fail(OMOE_ERR_INVALID, fn, "a tensor is not aligned to its element type");
+        if (!out) continue;
+        if (out[i].count != g.count || out[i].dtype != g.dtype) return ops_fail(OMOE_ERR_INVALID, fn, "out[i] must have the count and dtype of grads[i]");
+        if (g.count > 0 && !out[i].ptr) return ops_fail(OMOE_ERR_INVALID, fn, "null tensor");
+        if (misaligned(out[i].ptr, elem)) return ops_fail(OMOE_ERR_INVALID, fn, "a tensor is not aligned to its element type");
+    }
+    if (!writes || n == 0) return OMOE_OK;
+    Span *s = static_cast<Span *>(malloc(sizeof(Span) * 2 * (size_t)n));
+    if (!s) return ops_fail(OMOE_ERR_NOMEM, fn, "out of host memory");
+    const int m = spans_of(out ? out : grads, n, s);
+    bool bad = false;
+    for (int i = 1; i < m; i++) bad = bad || s[i].lo < s[i - 1].hi;
+    if (out && !bad) {  // a gradient may be met by its own output alone, and only where it starts
+        Span *g = s + n;
+        const int mg = spans_of(grads, n, g);
+        for (int i = 0, j = 0; i < mg && !bad; i++) {
+            while (j < m && s[j].hi <= g[i].lo) j++;
+            for (int q = j; q < m && s[q].lo < g[i].hi; q++) bad = bad || !(s[q].i == g[i].i && s[q].lo == g[i].lo);
+        }
+    }
+    free(s);
+    return bad ? ops_fail(OMOE_ERR_INVALID, fn, "tensors of the list overlap") : OMOE_OK;
+}
+
+int grid_of(int chunks, int sms) {
+    const int most = sms * 4 < kSlots ? sms * 4 : kSlots;
+    return chunks < most ? chunks : most;
+}
+
+// Launches f(table, blocks, is it the first) for the tensors of the list, as many at a time as a table takes.
+template <int N, typename F>
+cudaError_t tables(const omoe_tensor *grads, const omoe_tensor *out, int n, int sms, F f) {
+    Table<N> t;
+    bool first = true;
+    for (int i = 0; i < n;) {
+        t.n = 0;
+        int64_t chunks = 0;
+        for (; i < n && t.n < N; i++) {
+            if (grads[i].count == 0) continue;
+            const int64_t c = (grads[i].count + kChunkElems - 1) / kChunkElems;
+            if (chunks + c > INT32_MAX) break;  // never for the first: count <= 2^42
+            t.e[t.n++] = {grads[i].ptr, out ? out[i].ptr : grads[i].ptr, grads[i].count, (int32_t)chunks, grads[i].dtype};
+            chunks += c;
+        }
+        if (t.n == 0) break;
+        t.chunks = (int32_t)chunks;
+        cudaError_t e = f(t, grid_of(t.chunks, sms), first);
+        if (e != cudaSuccess) return e;
+        first = false;
+    }
+    return cudaSuccess;
+}
+
+int used(const omoe_tensor *t, int n) {
+    int m = 0;
+    for (int i = 0; i < n; i++) m += t[i].count > 0;
+    return m;
+}
+
+// Blocks' sums of squares into the workspace; *slots is how many there are.
+cudaError_t launch_squares(const omoe_tensor *grads, int n, double *ws, int sms, cudaStream_t s, int *slots) {
+    *slots = 0;
+    auto go = [&](const auto &t, int blocks, bool first) {
+        using Tab = std::remove_cv_t<std::remove_reference_t<decltype(t)>>;
+        constexpr int N = sizeof(Tab::e) / sizeof(Entry);
+        if (first) *slots = blocks;
+        // later tables add to the slots of the first one
+        const int b = first ? blocks : (blocks < *slots ? blocks : *slots);
+        return launch_ex(grad_squares_kernel<N>, dim3(b), dim3(kThreads), 0, s, ops_pdl(), t, ws, first ? 0 : 1);
+    };
+    return used(grads, n) <= kFew ? tables<kFew>(grads, nullptr, n, sms, go) : tables<kMany>(grads, nullptr, n, sms, go);
+}
+
+cudaError_t launch_scale(const omoe_tensor *grads, const omoe_tensor *out, int n, const double *ws, int slots, const float *norm_in,
+                         float *norm_out, float max_norm, int sms, cudaStream_t s) {
+    auto go = [&](const auto &t, int blocks, bool first) {
+        using Tab = std::remove_cv_t<std::remove_reference_t<decltype(t)>>;
+        constexpr int N = sizeof(Tab::e) / sizeof(Entry);
+        return launch_ex(grad_scale_kernel<N>, dim3(blocks), dim3(kThreads), 0, s, ops_pdl(), t, ws, slots, norm_in,
+                         first ? norm_out : nullptr, max_norm, out ? 0 : 1);
+    };
+    return used(grads, n) <= kFew ? tables<kFew>(grads, out, n, sms, go) : tables<kMany>(grads, out, n, sms, go);
+}
+
+const char *norm_args_wrong(const float *norm, const void *ws, int64_t bytes) {
+    if (!norm || misaligned(norm, 4)) return "norm_dev is null or misaligned";
+    if (!ws || misaligned(ws, 16) || bytes < OMOE_GRAD_WORKSPACE_BYTES) return "the workspace is missing, misaligned or too small";
+    return nullptr;
+}
+
+}  // namespace
+}  // namespace omoe
+
+using namespace omoe;
+
+extern "C" {
+
+int omoe_grad_norm(const omoe_tensor *grads, int32_t n, float *norm_dev, void *workspace_dev, int64_t workspace_bytes,
+                   void *cuda_stream) {
+    const char *fn = "omoe_grad_norm";
+    if (int rc = check_list(grads, nullptr, n, false, fn)) return rc;
+    if (const char *bad = norm_args_wrong(norm_dev, workspace_dev, workspace_bytes)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
+    const int sms = ops_sm_count();
+    if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    double *ws = static_cast<double *>(workspace_dev);
+    int slots = 0;
+    cudaError_t e = launch_squares(grads, n, ws, sms, s, &slots);
+    if (e == cudaSuccess) e = launch_ex(grad_norm_kernel, dim3(1), dim3(kThreads), 0, s, ops_pdl(), ws, slots, norm_dev);
+    return ops_launched(e, fn);
+}
+
+int omoe_grad_scale(const omoe_tensor *grads, const omoe_tensor *out, int32_t n, const float *norm_dev, float max_norm,
+                    void *cuda_stream) {
+    const char *fn = "omoe_grad_scale";
+    if (int rc = check_list(grads, out, n, true, fn)) return rc;
+    if (!norm_dev || misaligned(norm_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "norm_dev is null or misaligned");
+    if (!(max_norm >= 0.f)) return ops_fail(OMOE_ERR_INVALID, fn, "max_norm must not be negative");
+    const int sms = ops_sm_count();
+    if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
+    return ops_launched(launch_scale(grads, out, n, nullptr, 0, norm_dev, nullptr, max_norm, sms, static_cast<cudaStream_t>(cuda_stream)), fn);
+}
+
+int omoe_grad_clip(const omoe_tensor *grads, const omoe_tensor *out, int32_t n, float max_norm, float *norm_dev,
+                   void *workspace_dev, int64_t workspace_bytes, void *cuda_stream) {
+    const char *fn = "omoe_grad_clip";
+    if (int rc = check_list(grads, out, n, true, fn)) return rc;
+    if (const char *bad = norm_args_wrong(norm_dev, workspace_dev, workspace_bytes)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
+    if (!(max_norm >= 0.f)) return ops_fail(OMOE_ERR_INVALID, fn, "max_norm must not be negative");
+    const int sms = ops_sm_count();
+    if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    double *ws = static_cast<double *>(workspace_dev);
+    if (used(grads, n) == 0) return ops_launched(launch_ex(grad_norm_kernel, dim3(1), dim3(kThreads), 0, s, ops_pdl(), ws, 0, norm_dev), fn);
+    int slots = 0;
+    cudaError_t e = launch_squares(grads, n, ws, sms, s, &slots);
+    if (e == cudaSuccess) e = launch_scale(grads, out, n, ws, slots, nullptr, norm_dev, max_norm, sms, s);
+    return ops_launched(e, fn);
+}
+
+}  // extern "C"

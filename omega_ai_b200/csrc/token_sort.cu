@@ -1,0 +1,507 @@
+// Token rows sorted by expert and back, with weights applied, and the gradients of both.
+//
+// The plan is a stable counting sort of the T*top_k picks by expert.  The rows are moved by the inverse of it (the row
+// of every pick), so that a token's row is read once for all its picks and a sum over a token's picks runs in pick
+// order: nothing here needs an atomic, and the same inputs give the same bits.
+#include "ops.cuh"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
+namespace omoe {
+
+namespace {
+
+constexpr int64_t kRowsMax = 0x7fff0000;  // row numbers, and a block's worth beyond them, fit 32 bits
+constexpr int kPlanWarps = 32;
+constexpr int kPlanBatch = 8;    // picks a lane loads together
+constexpr int kPlanCtasMax = 8;  // the portable cluster size
+
+// One cluster does the whole plan.  Every warp owns a contiguous run of picks and counts its picks of every expert in
+// shared memory (lanes with the same expert are found with a match, the lowest adds them up); after sums over the
+// warps and, through distributed shared memory, over the CTAs every warp knows where its first pick of each
+// expert goes, walks its run again and numbers the picks.  Bound by latency: the two walks and the barriers.
+__global__ void __launch_bounds__(kPlanWarps * 32)
+sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int rows_cap, int warp_run,
+                 int32_t *__restrict__ pos, int32_t *__restrict__ perm, int32_t *__restrict__ counts,
+                 int32_t *__restrict__ offsets) {
+    extern __shared__ int32_t sm[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int nw = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t *s_total = sm;             // [E] this CTA's picks of every expert, read by the others
+    int32_t *s_count = s_total + E;    // [E] all picks
+    int32_t *s_start = s_count + E;    // [E+1] first row of every expert
+    int32_t *s_hist = s_start + E + 1; // [warps][E]
+    int32_t *hist = s_hist + warp * E;
+    const int ctas = cluster.num_blocks(), cta = cluster.block_rank();
+
+    pdl_trigger();
+    for (int e = lane; e < E; e += 32) hist[e] = 0;
+    const int64_t lo64 = (int64_t)(cta * nw + warp) * warp_run;
+    const int lo = (int)min((int64_t)n, lo64), hi = (int)min((int64_t)n, lo64 + warp_run);
+    pdl_wait();
+    __syncwarp();
+    int32_t key[kPlanBatch];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kPlanBatch; u++) {
+            const int i = i0 + u * 32 + lane;
+            const int e = i < hi ? idx[i] : -1;
+            key[u] = e >= 0 && e < E ? e : -1;
+        }
+    };
+    for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
+        fetch(i0);
+#pragma unroll
+        for (int u = 0; u < kPlanBatch; u++) {
+            if (i0 + u * 32 >= hi) break;
+            const uint32_t same = __match_any_sync(0xffffffffu, key[u]);
+            if (key[u] >= 0 && lane == __ffs(same) - 1) hist[key[u]] += __popc(same);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int run = 0;
+#pragma unroll 4
+        for (int w = 0; w < nw; w++) {
+            const int c = s_hist[w * E + e];
+            s_hist[w * E + e] = run;
+            run += c;
+        }
+        s_total[e] = run;
+    }
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int before = 0, all = 0;
+        for (int c = 0; c < ctas; c++) {
+            const int v = c == cta ? s_total[e] : cluster.map_shared_rank(s_total, c)[e];
+            if (c < cta) before += v;
+            all += v;
+        }
+        s_count[e] = all;
+        s_start[e] = before;  // the expert's first row is added below
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int row = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane;
+            const int c = e < E ? s_count[e] : 0, p = (c + align - 1) / align * align;
+            int inc = p;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            if (e < E) {
+                const int first = row + inc - p;
+                s_start[e] += first;
+                if (cta == 0) {
+                    counts[e] = c;
+                    offsets[e] = first;
+                }
+                // padding rows have no pick; the CTAs share the experts
+                if (e % ctas == cta)
+                    for (int r = first + c; r < first + p && r < rows_cap; r++) perm[r] = -1;
+            }
+            row += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) {
+            s_start[E] = row;
+            if (cta == 0) offsets[E] = row;
+        }
+    }
+    __syncthreads();
+    for (int64_t r = (int64_t)s_start[E] + cta * blockDim.x + threadIdx.x; r < rows_cap; r += ctas * blockDim.x) perm[r] = -1;
+    for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
+        if (warp_run > kPlanBatch * 32) fetch(i0);
+#pragma unroll
+        for (int u = 0; u < kPlanBatch; u++) {
+            const int i = i0 + u * 32 + lane, e = key[u];
+            if (i0 + u * 32 >= hi) break;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            int row = -1;
+            if (e >= 0) row = s_start[e] + hist[e] + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (e >= 0 && lane == __ffs(same) - 1) hist[e] += __popc(same);
+            __syncwarp();
+            if (i < hi) {
+                pos[i] = row;
+                if (row >= 0 && row < rows_cap) perm[row] = i;
+            }
+        }
+    }
+    if (ctas > 1) cluster.sync();  // the others may still read this CTA's totals
+}
+
+// A warp takes one chunk of a token's columns: U vectors per lane.
+template <int V>
+constexpr int kChunk = 32 * V * (V == 8 ? 4 : 8);
+
+// The rows of a token's picks, a pick per lane; picks without a row, or with one that no plan makes, are negative.
+__device__ __forceinline__ int pick_row(const int32_t *pos, int64_t t, int k, int lane, int rows_cap) {
+    int r = -1;
+    if (lane < k) r = pos[t * k + lane];
+    return r < rows_cap ? r : -1;
+}
+
+// Zeros for the padding rows of expert e, columns [c0, c1), by one warp.
+template <typename T, int V>
+__device__ __forceinline__ void zero_padding(T *rows, int64_t ld, const int32_t *counts, const int32_t *offsets, int e, int c0,
+                                             int c1, int lane, int rows_cap) {
+    const int first = offsets[e] + counts[e], last = min(offsets[e + 1], rows_cap);
+    Frag<T, V> z;
+    z.zero();
+    if (first < 0) return;
+    for (int r = first; r < last; r++)
+        for (int c = c0 + lane * V; c < c1; c += 32 * V) z.store(rows + (int64_t)r * ld + c);
+}
+
+// xs[pos] = x: a warp reads a chunk of a token's row once and stores it for every pick.  HBM bound.
+template <typename XT, typename OT, int V>
+__global__ void __launch_bounds__(256)
+sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int64_t ldxs, const int32_t *__restrict__ pos,
+                 const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int T, int k, int E, int d,
+                 int n_chunks, int rows_cap) {
+    constexpr int U = kChunk<V> / (32 * V);
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t t = item / n_chunks;
+    const int c0 = (int)(item % n_chunks) * kChunk<V> + lane * V;
+    pdl_trigger();
+    pdl_wait();
+    if (t >= T) {
+        if (t - T < E) zero_padding<OT, V>(xs, ldxs, counts, offsets, (int)(t - T), c0 - lane * V, min(d, c0 - lane * V + kChunk<V>), lane, rows_cap);
+        return;
+    }
+    const int r = pick_row(pos, t, k, lane, rows_cap);
+    uint32_t picks = __ballot_sync(0xffffffffu, r >= 0);
+    if (!picks) return;
+    Frag<XT, V> in[U];
+    Frag<OT, V> out[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (c0 + u * 32 * V < d) in[u].load(x + t * ldx + c0 + u * 32 * V);
+#pragma unroll
+    for (int u = 0; u < U; u++) convert(in[u], out[u]);
+    for (; picks; picks &= picks - 1) {
+        OT *to = xs + (int64_t)__shfl_sync(0xffffffffu, r, __ffs(picks) - 1) * ldxs;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u * 32 * V < d) out[u].store(to + c0 + u * 32 * V);
+    }
+}
+
+// y[t] = sum over the picks of w * ys[pos] (W) or of ys[pos]: a warp per chunk of a token's columns, two picks' loads in
+// flight.  fp32 sums in pick order.  HBM bound.
+template <typename XT, typename OT, int V, bool W>
+__global__ void __launch_bounds__(256)
+unsort_rows_kernel(const XT *__restrict__ ys, int64_t ldys, OT *__restrict__ y, int64_t ldy, const int32_t *__restrict__ pos,
+                   const float *__restrict__ w, int T, int k, int d, int n_chunks, int rows_cap) {
+    constexpr int U = kChunk<V> / (32 * V);
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t t = item / n_chunks;
+    const int c0 = (int)(item % n_chunks) * kChunk<V> + lane * V;
+    pdl_trigger();
+    pdl_wait();
+    if (t >= T) return;
+    const int r = pick_row(pos, t, k, lane, rows_cap);
+    float wl = 1.f;
+    if (W && lane < k) wl = w[t * k + lane];
+    uint32_t picks = __ballot_sync(0xffffffffu, r >= 0);
+    float acc[U][V];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[u][i] = 0.f;
+    while (picks) {
+        const int j0 = __ffs(picks) - 1;
+        picks &= picks - 1;
+        const int j1 = picks ? __ffs(picks) - 1 : -1;
+        picks &= picks - 1;  // stays 0 where it is
+        Frag<XT, V> a[U], b[U];
+        const XT *p0 = ys + (int64_t)__shfl_sync(0xffffffffu, r, j0) * ldys;
+        const XT *p1 = ys + (int64_t)__shfl_sync(0xffffffffu, r, j1 < 0 ? j0 : j1) * ldys;
+        const float w0 = __shfl_sync(0xffffffffu, wl, j0), w1 = __shfl_sync(0xffffffffu, wl, j1 < 0 ? j0 : j1);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u * 32 * V < d) {
+                a[u].load(p0 + c0 + u * 32 * V);
+                if (j1 >= 0) b[u].load(p1 + c0 + u * 32 * V);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u * 32 * V < d) {
+                float v[V];
+                a[u].get(v);
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[u][i] = W ? fmaf(w0, v[i], acc[u][i]) : acc[u][i] + v[i];
+                if (j1 >= 0) {
+                    b[u].get(v);
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[u][i] = W ? fmaf(w1, v[i], acc[u][i]) : acc[u][i] + v[i];
+                }
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (c0 + u * 32 * V < d) {
+            Frag<OT, V> o;
+            o.set(acc[u]);
+            o.store(y + t * ldy + c0 + u * 32 * V);
+        }
+}
+
+// dys[pos] = w * dy and dw = <dy, ys[pos]>: a block per token reads dy once; a thread's columns are added up for every
+// pick in registers, then over the warp and the block in a fixed order.  K bounds k.  HBM bound.
+template <typename DT, typename YT, int V, int K>
+__global__ void __launch_bounds__(512)
+unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict__ ys, int64_t ldys, YT *__restrict__ dys,
+                  int64_t lddys, const int32_t *__restrict__ pos, const int32_t *__restrict__ counts,
+                  const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int E,
+                  int d, int rows_cap) {
+    __shared__ float s_dot[16][K];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int64_t t = blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    if (t >= T) {  // a block per expert for its padding rows, a warp per part of the columns
+        const int part = ((d + nw - 1) / nw + V * 32 - 1) / (V * 32) * (V * 32), c0 = warp * part;
+        if (c0 < d) zero_padding<YT, V>(dys, lddys, counts, offsets, (int)(t - T), c0, min(d, c0 + part), lane, rows_cap);
+        return;
+    }
+    int row[K];
+    float wt[K], dot[K];
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        row[j] = j < k ? pos[t * k + j] : -1;
+        if (row[j] >= rows_cap) row[j] = -1;
+        wt[j] = w && j < k ? w[t * k + j] : 1.f;
+        dot[j] = 0.f;
+    }
+    for (int c = threadIdx.x * V; c < d; c += blockDim.x * V) {
+        Frag<DT, V> g;
+        Frag<YT, V> y[K], o;
+        g.load(dy + t * lddy + c);
+        if (dw)
+#pragma unroll
+            for (int j = 0; j < K; j++)
+                if (row[j] >= 0) y[j].load(ys + (int64_t)row[j] * ldys + c);
+        float gv[V], v[V];
+        g.get(gv);
+#pragma unroll
+        for (int j = 0; j < K; j++)
+            if (row[j] >= 0) {
+#pragma unroll
+                for (int i = 0; i < V; i++) v[i] = wt[j] * gv[i];
+                o.set(v);
+                o.store(dys + (int64_t)row[j] * lddys + c);
+                if (dw) {
+                    y[j].get(v);
+#pragma unroll
+                    for (int i = 0; i < V; i++) dot[j] = fmaf(gv[i], v[i], dot[j]);
+                }
+            }
+    }
+    if (!dw) return;
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+#pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
+        if (lane == 0) s_dot[warp][j] = dot[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < k) {
+        float sum = 0.f;
+        for (int i = 0; i < nw; i++) sum += s_dot[i][threadIdx.x];
+        dw[t * k + threadIdx.x] = sum;
+    }
+}
+
+const char *plan_wrong(const omoe_sort *p) {
+    if (!p) return "null plan";
+    if (p->n_tokens < 0 || p->top_k < 1 || p->n_experts < 1 || p->row_align < 1) return "bad sizes in the plan";
+    if (!p->counts || !p->offsets || (p->n_tokens > 0 && (!p->pos || !p->perm))) return "null buffer in the plan";
+    if (misaligned(p->pos, 4) || misaligned(p->perm, 4) || misaligned(p->counts, 4) || misaligned(p->offsets, 4))
+        return "the plan's buffers must be 4-byte aligned";
+    return nullptr;
+}
+
+// The plan of a call on rows: status, with the text set.
+int check_plan(const omoe_sort *p, const char *fn) {
+    if (const char *bad = plan_wrong(p)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
+    const int64_t need = omoe_sort_rows_cap(p->n_tokens, p->top_k, p->n_experts, p->row_align);
+    if (need < 0) return ops_fail((int)need, fn, "the plan's sizes are beyond the limits");
+    if (p->rows_cap < need) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "rows_cap is smaller than omoe_sort_rows_cap()");
+    if (p->rows_cap > kRowsMax) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "rows_cap is beyond the limit");
+    return OMOE_OK;
+}
+
+int check_rows(const Rows *const *m, int n, int n_out, const char *fn) {
+    for (int i = 0; i < n; i++)
+        if (const char *bad = rows_wrong(*m[i])) return ops_fail(OMOE_ERR_INVALID, fn, bad);
+    for (int i = 0; i < n_out; i++)  // outputs come first
+        for (int j = i + 1; j < n; j++)
+            if (rows_overlap(*m[i], *m[j])) return ops_fail(OMOE_ERR_INVALID, fn, "an output overlaps another buffer");
+    return OMOE_OK;
+}
+
+template <int V>
+int64_t row_items(int64_t T, int d) { return T * ((d + kChunk<V> - 1) / kChunk<V>); }
+
+}  // namespace
+}  // namespace omoe
+
+using namespace omoe;
+
+extern "C" {
+
+int64_t omoe_sort_rows_cap(int32_t n_tokens, int32_t top_k, int32_t n_experts, int32_t row_align) {
+    if (n_tokens < 0 || top_k < 1 || n_experts < 1 || row_align < 1) return OMOE_ERR_INVALID;
+    if (n_experts > OMOE_SORT_MAX_EXPERTS || top_k > kMaxTopK) return OMOE_ERR_TOO_LARGE;
+    const int64_t n = (int64_t)n_tokens * top_k, padded = n < n_experts ? n : n_experts;
+    const int64_t rows = (n + padded * (row_align - 1) + row_align - 1) / row_align * row_align;
+    return rows > kRowsMax ? OMOE_ERR_TOO_LARGE : rows;
+}
+
+int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cuda_stream) {
+    const char *fn = "omoe_sort_plan";
+    if (int rc = check_plan(plan, fn)) return rc;
+    if (plan->n_tokens > 0 && !topk_idx_dev) return ops_fail(OMOE_ERR_INVALID, fn, "null buffer");
+    if (misaligned(topk_idx_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "topk_idx_dev must be 4-byte aligned");
+    const int n = plan->n_tokens * plan->top_k, E = plan->n_experts;  // below 2^31: check_plan
+    // a warp takes 64 picks before a second CTA joins, and up to eight CTAs share the rest
+    int warps = ceil_div(n, 64), ctas = 1;
+    while (ctas < kPlanCtasMax && warps > ctas * kPlanWarps) ctas *= 2;
+    warps = warps < 1 ? 1 : warps > kPlanWarps ? kPlanWarps : warps;
+    const int64_t run = round_up(((int64_t)n + ctas * warps - 1) / (ctas * warps), 32);
+    const size_t smem = sizeof(int32_t) * ((size_t)E * (3 + warps) + 1);
+    static PerDeviceOnce once;
+    bool *done = once.slot();
+    if (!done || !*done) {
+        const size_t most = sizeof(int32_t) * ((size_t)OMOE_SORT_MAX_EXPERTS * (3 + kPlanWarps) + 1);
+        cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (e != cudaSuccess) return ops_launched(e, fn);
+        if (done) *done = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(cuda_stream);
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = ops_pdl() ? 2 : 1;
+    return ops_launched(cudaLaunchKernelEx(&cfg, sort_plan_kernel, topk_idx_dev, n, E, (int)plan->row_align,
+                                           (int)plan->rows_cap, (int)run, plan->pos, plan->perm, plan->counts,
+                                           plan->offsets), fn);
+}
+
+int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_t x_dtype, void *xs_dev, int64_t ldxs,
+                   int32_t xs_dtype, int32_t d, void *cuda_stream) {
+    const char *fn = "omoe_sort_rows";
+    if (int rc = check_plan(plan, fn)) return rc;
+    const int T = plan->n_tokens, E = plan->n_experts;
+    const Rows x = {x_dev, ldx, x_dtype, T, d}, xs = {xs_dev, ldxs, xs_dtype, plan->rows_cap, d};
+    const Rows *all[] = {&xs, &x};
+    if (int rc = check_rows(all, 2, 1, fn)) return rc;
+    if (T == 0) return ops_ok();
+    const bool vec = rows_vector(x) && rows_vector(xs);
+    const int64_t tokens = T + (plan->row_align > 1 ? E : 0);  // an expert's padding is one more "token"
+    const int64_t blocks = ((vec ? row_items<8>(tokens, d) : row_items<1>(tokens, d)) + 7) / 8;
+    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
+    return ops_launched(by_types(x_dtype, xs_dtype, [&](auto *xt, auto *ot) {
+        using XT = std::remove_pointer_t<decltype(xt)>;
+        using OT = std::remove_pointer_t<decltype(ot)>;
+        auto go = [&](auto kern, int chunk) {
+            return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
+                             static_cast<const XT *>(x_dev), ldx, static_cast<OT *>(xs_dev), ldxs, plan->pos, plan->counts,
+                             plan->offsets, T, plan->top_k, E, d, ceil_div(d, chunk), (int)plan->rows_cap);
+        };
+        return vec ? go(sort_rows_kernel<XT, OT, 8>, kChunk<8>) : go(sort_rows_kernel<XT, OT, 1>, kChunk<1>);
+    }), fn);
+}
+
+static int unsort(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32_t ys_dtype, const float *w_dev, void *y_dev,
+                  int64_t ldy, int32_t y_dtype, int32_t d, void *cuda_stream, const char *fn) {
+    if (int rc = check_plan(plan, fn)) return rc;
+    const int T = plan->n_tokens;
+    const Rows y = {y_dev, ldy, y_dtype, T, d}, ys = {ys_dev, ldys, ys_dtype, T ? plan->rows_cap : 0, d};
+    const Rows *all[] = {&y, &ys};
+    if (int rc = check_rows(all, 2, 1, fn)) return rc;
+    if (misaligned(w_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
+    if (T == 0) return ops_ok();
+    const bool vec = rows_vector(y) && rows_vector(ys);
+    const int64_t blocks = ((vec ? row_items<8>(T, d) : row_items<1>(T, d)) + 7) / 8;
+    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
+    return ops_launched(by_types(ys_dtype, y_dtype, [&](auto *xt, auto *ot) {
+        using XT = std::remove_pointer_t<decltype(xt)>;
+        using OT = std::remove_pointer_t<decltype(ot)>;
+        auto go = [&](auto kern, int chunk) {
+            return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
+                             static_cast<const XT *>(ys_dev), ldys, static_cast<OT *>(y_dev), ldy, plan->pos, w_dev, T,
+                             plan->top_k, d, ceil_div(d, chunk), (int)plan->rows_cap);
+        };
+        if (vec) return w_dev ? go(unsort_rows_kernel<XT, OT, 8, true>, kChunk<8>) : go(unsort_rows_kernel<XT, OT, 8, false>, kChunk<8>);
+        return w_dev ? go(unsort_rows_kernel<XT, OT, 1, true>, kChunk<1>) : go(unsort_rows_kernel<XT, OT, 1, false>, kChunk<1>);
+    }), fn);
+}
+
+int omoe_sort_rows_backward(const omoe_sort *plan, const void *dxs_dev, int64_t lddxs, int32_t dxs_dtype, void *dx_dev,
+                            int64_t lddx, int32_t dx_dtype, int32_t d, void *cuda_stream) {
+    return unsort(plan, dxs_dev, lddxs, dxs_dtype, nullptr, dx_dev, lddx, dx_dtype, d, cuda_stream, "omoe_sort_rows_backward");
+}
+
+int omoe_unsort_rows(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32_t ys_dtype, const float *w_dev, void *y_dev,
+                     int64_t ldy, int32_t y_dtype, int32_t d, void *cuda_stream) {
+    return unsort(plan, ys_dev, ldys, ys_dtype, w_dev, y_dev, ldy, y_dtype, d, cuda_stream, "omoe_unsort_rows");
+}
+
+int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t lddy, int32_t dy_dtype, const void *ys_dev,
+                              int64_t ldys, int32_t ys_dtype, const float *w_dev, void *dys_dev, int64_t lddys, float *dw_dev,
+                              int32_t d, void *cuda_stream) {
+    const char *fn = "omoe_unsort_rows_backward";
+    if (int rc = check_plan(plan, fn)) return rc;
+    const int T = plan->n_tokens, E = plan->n_experts, k = plan->top_k;
+    const Rows dys = {dys_dev, lddys, ys_dtype, T ? plan->rows_cap : 0, d}, dy = {dy_dev, lddy, dy_dtype, T, d};
+    const Rows ys = {ys_dev, ldys, ys_dtype, T && dw_dev ? plan->rows_cap : 0, d};
+    const Rows *all[] = {&dys, &dy, &ys};
+    if (int rc = check_rows(all, dw_dev ? 3 : 2, 1, fn)) return rc;
+    if (misaligned(w_dev, 4) || misaligned(dw_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
+    if (T == 0) return ops_ok();
+    const int64_t blocks = (int64_t)T + (plan->row_align > 1 ? E : 0);
+    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
+    const bool vec = rows_vector(dys) && rows_vector(dy) && (!dw_dev || rows_vector(ys));
+    const int per = vec ? 8 : 1;
+    int threads = 64;
+    while (threads < 512 && threads * per * 2 < d) threads *= 2;
+    return ops_launched(by_types(dy_dtype, ys_dtype, [&](auto *dt, auto *yt) {
+        using DT = std::remove_pointer_t<decltype(dt)>;
+        using YT = std::remove_pointer_t<decltype(yt)>;
+        auto go = [&](auto kern) {
+            return launch_ex(kern, dim3((unsigned)blocks), dim3(threads), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
+                             static_cast<const DT *>(dy_dev), lddy, static_cast<const YT *>(ys_dev), ldys,
+                             static_cast<YT *>(dys_dev), lddys, plan->pos, plan->counts, plan->offsets, w_dev, dw_dev, T, k, E,
+                             d, (int)plan->rows_cap);
+        };
+        auto by_k = [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            if (k <= 2) return go(unsort_bwd_kernel<DT, YT, V, 2>);
+            if (k <= 4) return go(unsort_bwd_kernel<DT, YT, V, 4>);
+            if (k <= 8) return go(unsort_bwd_kernel<DT, YT, V, 8>);
+            return go(unsort_bwd_kernel<DT, YT, V, 16>);
+        };
+        return vec ? by_k(std::integral_constant<int, 8>()) : by_k(std::integral_constant<int, 1>());
+    }), fn);
+}
+
+}  // extern "C"

@@ -69,4 +69,53 @@ public final class OmoeNative {
     public static native int epExport(long handle, byte[] blob320);
 
     public static native int epImport(long handle, byte[] allBlobs);
+
+    /** Text of the last failure of the operators below on this thread. */
+    public static native String opsError();
+
+    /** omoe_sort_rows_cap: rows of the sorted buffers, or a negative status. */
+    public static native long sortRowsCap(int tokens, int topK, int nExperts, int rowAlign);
+
+    /**
+     * omoe_sort_plan.  plan = {tokens, topK, nExperts, rowAlign, rowsCap, pos, perm, counts, offsets}: sizes, then device
+     * addresses of int32 buffers [tokens * topK], [rowsCap], [nExperts], [nExperts + 1].
+     */
+    public static native int sortPlan(long[] plan, long topkIdxDev);
+
+    /** omoe_sort_rows: token rows to their places by expert. */
+    public static native int sortRows(long[] plan, long xDev, long ldx, int xDtype, long xsDev, long ldxs, int xsDtype, int d);
+
+    public static native int sortRowsBackward(long[] plan, long dxsDev, long lddxs, int dxsDtype, long dxDev, long lddx,
+                                              int dxDtype, int d);
+
+    /** omoe_unsort_rows: weighted sum of every token's rows; wDev may be 0. */
+    public static native int unsortRows(long[] plan, long ysDev, long ldys, int ysDtype, long wDev, long yDev, long ldy,
+                                        int yDtype, int d);
+
+    public static native int unsortRowsBackward(long[] plan, long dyDev, long lddy, int dyDtype, long ysDev, long ldys,
+                                                int ysDtype, long wDev, long dysDev, long lddys, long dwDev, int d);
+
+    /** omoe_layer_norm; gammaDev, betaDev, meanDev and rstdDev are fp32 device addresses or 0. */
+    public static native int layerNorm(long xDev, long ldx, int xDtype, long gammaDev, long betaDev, float eps, long yDev,
+                                       long ldy, int yDtype, long meanDev, long rstdDev, int tokens, int d);
+
+    public static native long layerNormBackwardWorkspace(int tokens, int d);
+
+    public static native int layerNormBackward(long dyDev, long lddy, int dyDtype, long xDev, long ldx, int xDtype,
+                                               long gammaDev, long meanDev, long rstdDev, long dxDev, long lddx,
+                                               long dgammaDev, long dbetaDev, int tokens, int d, long workspaceDev,
+                                               long workspaceBytes);
+
+    /** omoe_grad_norm over the tensors (device addresses, element counts, dtypes); workspace of GRAD_WORKSPACE_BYTES. */
+    public static native int gradNorm(long[] grads, long[] counts, int[] dtypes, long normDev, long workspaceDev,
+                                      long workspaceBytes);
+
+    /** omoe_grad_scale, in place. */
+    public static native int gradScale(long[] grads, long[] counts, int[] dtypes, long normDev, float maxNorm);
+
+    /** omoe_grad_clip, in place. */
+    public static native int gradClip(long[] grads, long[] counts, int[] dtypes, float maxNorm, long normDev,
+                                      long workspaceDev, long workspaceBytes);
+
+    public static final int GRAD_WORKSPACE_BYTES = 16384;
 }

@@ -15,6 +15,7 @@
 
 #ifdef OMOE_HAVE_JNI
 #include <jni.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include "omoe.h"
@@ -149,6 +150,122 @@ JFN(jint, epImport)(JNIEnv *env, jclass c, jlong h, jbyteArray blobs) {
     jbyte *p = (*env)->GetByteArrayElements(env, blobs, NULL);
     int rc = omoe_ep_import((omoe_handle *)(intptr_t)h, p);
     (*env)->ReleaseByteArrayElements(env, blobs, p, JNI_ABORT);
+    return rc;
+}
+/* ---- operators without a handle ---- */
+#define P(a) ((void *)(intptr_t)(a))
+
+JFN(jstring, opsError)(JNIEnv *env, jclass c) { return (*env)->NewStringUTF(env, omoe_ops_error()); }
+
+JFN(jlong, sortRowsCap)(JNIEnv *env, jclass c, jint T, jint k, jint E, jint align) {
+    return omoe_sort_rows_cap(T, k, E, align);
+}
+
+/* The plan's sizes and addresses, 9 longs; false where there are fewer or a size does not fit. */
+static int read_plan(JNIEnv *env, jlongArray plan, omoe_sort *p) {
+    if (!plan || (*env)->GetArrayLength(env, plan) < 9) return 0;
+    jlong *v = (*env)->GetLongArrayElements(env, plan, NULL);
+    if (!v) return 0;
+    int ok = 1;
+    for (int i = 0; i < 4; i++) ok = ok && v[i] >= INT32_MIN && v[i] <= INT32_MAX;
+    p->n_tokens = (int32_t)v[0]; p->top_k = (int32_t)v[1]; p->n_experts = (int32_t)v[2]; p->row_align = (int32_t)v[3];
+    p->rows_cap = v[4];
+    p->pos = (int32_t *)P(v[5]); p->perm = (int32_t *)P(v[6]); p->counts = (int32_t *)P(v[7]); p->offsets = (int32_t *)P(v[8]);
+    (*env)->ReleaseLongArrayElements(env, plan, v, JNI_ABORT);
+    return ok;
+}
+
+JFN(jint, sortPlan)(JNIEnv *env, jclass c, jlongArray plan, jlong idx) {
+    omoe_sort p;
+    return read_plan(env, plan, &p) ? omoe_sort_plan(&p, (const int32_t *)P(idx), NULL) : OMOE_ERR_INVALID;
+}
+
+JFN(jint, sortRows)(JNIEnv *env, jclass c, jlongArray plan, jlong x, jlong ldx, jint xdt, jlong xs, jlong ldxs, jint xsdt, jint d) {
+    omoe_sort p;
+    return read_plan(env, plan, &p) ? omoe_sort_rows(&p, P(x), ldx, xdt, P(xs), ldxs, xsdt, d, NULL) : OMOE_ERR_INVALID;
+}
+
+JFN(jint, sortRowsBackward)(JNIEnv *env, jclass c, jlongArray plan, jlong dxs, jlong lddxs, jint dxsdt, jlong dx, jlong lddx,
+                            jint dxdt, jint d) {
+    omoe_sort p;
+    return read_plan(env, plan, &p) ? omoe_sort_rows_backward(&p, P(dxs), lddxs, dxsdt, P(dx), lddx, dxdt, d, NULL) : OMOE_ERR_INVALID;
+}
+
+JFN(jint, unsortRows)(JNIEnv *env, jclass c, jlongArray plan, jlong ys, jlong ldys, jint ysdt, jlong w, jlong y, jlong ldy,
+                      jint ydt, jint d) {
+    omoe_sort p;
+    return read_plan(env, plan, &p) ? omoe_unsort_rows(&p, P(ys), ldys, ysdt, (const float *)P(w), P(y), ldy, ydt, d, NULL)
+                                    : OMOE_ERR_INVALID;
+}
+
+JFN(jint, unsortRowsBackward)(JNIEnv *env, jclass c, jlongArray plan, jlong dy, jlong lddy, jint dydt, jlong ys, jlong ldys,
+                              jint ysdt, jlong w, jlong dys, jlong lddys, jlong dw, jint d) {
+    omoe_sort p;
+    return read_plan(env, plan, &p) ? omoe_unsort_rows_backward(&p, P(dy), lddy, dydt, P(ys), ldys, ysdt, (const float *)P(w),
+                                                                P(dys), lddys, (float *)P(dw), d, NULL)
+                                    : OMOE_ERR_INVALID;
+}
+
+JFN(jint, layerNorm)(JNIEnv *env, jclass c, jlong x, jlong ldx, jint xdt, jlong gamma, jlong beta, jfloat eps, jlong y, jlong ldy,
+                     jint ydt, jlong mean, jlong rstd, jint T, jint d) {
+    return omoe_layer_norm(P(x), ldx, xdt, (const float *)P(gamma), (const float *)P(beta), eps, P(y), ldy, ydt, (float *)P(mean),
+                           (float *)P(rstd), T, d, NULL);
+}
+
+JFN(jlong, layerNormBackwardWorkspace)(JNIEnv *env, jclass c, jint T, jint d) { return omoe_layer_norm_backward_workspace(T, d); }
+
+JFN(jint, layerNormBackward)(JNIEnv *env, jclass c, jlong dy, jlong lddy, jint dydt, jlong x, jlong ldx, jint xdt, jlong gamma,
+                             jlong mean, jlong rstd, jlong dx, jlong lddx, jlong dgamma, jlong dbeta, jint T, jint d, jlong ws,
+                             jlong wsBytes) {
+    return omoe_layer_norm_backward(P(dy), lddy, dydt, P(x), ldx, xdt, (const float *)P(gamma), (const float *)P(mean),
+                                    (const float *)P(rstd), P(dx), lddx, (float *)P(dgamma), (float *)P(dbeta), T, d, P(ws),
+                                    wsBytes, NULL);
+}
+
+/* Host table of the tensors, to be freed; *n is -1 where the arrays do not agree or memory is short. */
+static omoe_tensor *read_tensors(JNIEnv *env, jlongArray ptrs, jlongArray counts, jintArray dtypes, jint *n) {
+    *n = -1;
+    if (!ptrs || !counts || !dtypes) return NULL;
+    jint m = (*env)->GetArrayLength(env, ptrs);
+    if ((*env)->GetArrayLength(env, counts) != m || (*env)->GetArrayLength(env, dtypes) != m) return NULL;
+    omoe_tensor *t = (omoe_tensor *)malloc(sizeof(omoe_tensor) * (size_t)(m > 0 ? m : 1));
+    if (!t) return NULL;
+    jlong *a = (*env)->GetLongArrayElements(env, ptrs, NULL), *b = (*env)->GetLongArrayElements(env, counts, NULL);
+    jint *d = (*env)->GetIntArrayElements(env, dtypes, NULL);
+    if (a && b && d) {
+        for (jint i = 0; i < m; i++) {
+            t[i].ptr = P(a[i]); t[i].count = b[i]; t[i].dtype = d[i]; t[i].reserved = 0;
+        }
+        *n = m;
+    }
+    if (a) (*env)->ReleaseLongArrayElements(env, ptrs, a, JNI_ABORT);
+    if (b) (*env)->ReleaseLongArrayElements(env, counts, b, JNI_ABORT);
+    if (d) (*env)->ReleaseIntArrayElements(env, dtypes, d, JNI_ABORT);
+    return t;
+}
+
+JFN(jint, gradNorm)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray dt, jlong norm, jlong ws, jlong wsBytes) {
+    jint m;
+    omoe_tensor *t = read_tensors(env, g, n, dt, &m);
+    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_norm(t, m, (float *)P(norm), P(ws), wsBytes, NULL);
+    free(t);
+    return rc;
+}
+
+JFN(jint, gradScale)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray dt, jlong norm, jfloat maxNorm) {
+    jint m;
+    omoe_tensor *t = read_tensors(env, g, n, dt, &m);
+    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_scale(t, NULL, m, (const float *)P(norm), maxNorm, NULL);
+    free(t);
+    return rc;
+}
+
+JFN(jint, gradClip)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray dt, jfloat maxNorm, jlong norm, jlong ws,
+                    jlong wsBytes) {
+    jint m;
+    omoe_tensor *t = read_tensors(env, g, n, dt, &m);
+    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_clip(t, NULL, m, maxNorm, (float *)P(norm), P(ws), wsBytes, NULL);
+    free(t);
     return rc;
 }
 #else

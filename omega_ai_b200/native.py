@@ -35,7 +35,12 @@ SYMBOLS = (
     "omoe_set_profiling", "omoe_get_stage_ms", "omoe_get_stage_ms_at", "omoe_ep_export", "omoe_ep_import",
     "omoe_route_noalloc", "omoe_route_noalloc_error",
     "omoe_ep_connect_local", "omoe_set_training", "omoe_backward", "omoe_backward_block", "omoe_get_weight_grads", "omoe_set_aux_loss", "omoe_get_aux_loss",
+    "omoe_ops_error", "omoe_sort_rows_cap", "omoe_sort_plan", "omoe_sort_rows", "omoe_sort_rows_backward", "omoe_unsort_rows",
+    "omoe_unsort_rows_backward", "omoe_layer_norm", "omoe_layer_norm_backward_workspace", "omoe_layer_norm_backward",
+    "omoe_grad_norm", "omoe_grad_scale", "omoe_grad_clip",
 )
+SORT_MAX_EXPERTS = 1024
+GRAD_WORKSPACE_BYTES = 16384
 NOALLOC_MAX_TOKENS = 4096
 
 
@@ -55,6 +60,19 @@ class Config(C.Structure):
         ("has_router_bias", C.c_int32), ("world", C.c_int32), ("rank", C.c_int32),
         ("recv_rows_max", C.c_int32), ("reserved", C.c_int32 * 5),
     ]
+
+
+class Sort(C.Structure):
+    """omoe_sort: sizes and device buffers of a plan of sorted tokens."""
+    _fields_ = [
+        ("n_tokens", C.c_int32), ("top_k", C.c_int32), ("n_experts", C.c_int32), ("row_align", C.c_int32),
+        ("rows_cap", C.c_int64), ("pos", C.c_void_p), ("perm", C.c_void_p), ("counts", C.c_void_p), ("offsets", C.c_void_p),
+    ]
+
+
+class TensorRef(C.Structure):
+    """omoe_tensor: a contiguous device tensor in a list of gradients."""
+    _fields_ = [("ptr", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
 def sources():
@@ -115,8 +133,27 @@ def lib():
     L.omoe_get_aux_loss.argtypes = [vp, C.POINTER(C.c_float)]
     L.omoe_route_noalloc_error.argtypes = []
     L.omoe_route_noalloc_error.restype = C.c_char_p
+    i64, f32, sort, refs = C.c_int64, C.c_float, C.POINTER(Sort), C.POINTER(TensorRef)
+    L.omoe_ops_error.argtypes = []
+    L.omoe_ops_error.restype = C.c_char_p
+    L.omoe_sort_rows_cap.argtypes = [i32, i32, i32, i32]
+    L.omoe_sort_rows_cap.restype = i64
+    L.omoe_sort_plan.argtypes = [sort, vp, vp]
+    for rows in (L.omoe_sort_rows, L.omoe_sort_rows_backward):
+        rows.argtypes = [sort, vp, i64, i32, vp, i64, i32, i32, vp]
+    L.omoe_unsort_rows.argtypes = [sort, vp, i64, i32, vp, vp, i64, i32, i32, vp]
+    L.omoe_unsort_rows_backward.argtypes = [sort, vp, i64, i32, vp, i64, i32, vp, vp, i64, vp, i32, vp]
+    L.omoe_layer_norm.argtypes = [vp, i64, i32, vp, vp, f32, vp, i64, i32, vp, vp, i32, i32, vp]
+    L.omoe_layer_norm_backward_workspace.argtypes = [i32, i32]
+    L.omoe_layer_norm_backward_workspace.restype = i64
+    L.omoe_layer_norm_backward.argtypes = [vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, vp, vp, i32, i32, vp, i64, vp]
+    L.omoe_grad_norm.argtypes = [refs, i32, vp, vp, i64, vp]
+    L.omoe_grad_scale.argtypes = [refs, refs, i32, vp, f32, vp]
+    L.omoe_grad_clip.argtypes = [refs, refs, i32, f32, vp, vp, i64, vp]
+    other = ("omoe_last_error", "omoe_route_noalloc_error", "omoe_ops_error", "omoe_sort_rows_cap",
+             "omoe_layer_norm_backward_workspace")
     for name in SYMBOLS:
-        if name not in ("omoe_last_error", "omoe_route_noalloc_error"):
+        if name not in other:
             getattr(L, name).restype = C.c_int
     _lib = L
     return L

@@ -1,0 +1,92 @@
+"""The operators in a row, as a training step uses them around experts of its own: layer norm, routing, rows to the experts,
+a product per expert, weighted rows back, the backward pass, gradient clipping.  The gradients are compared with
+64-bit automatic differentiation of the same step on the routing the library chose.
+
+fp32 throughout.  A gradient passes seven operators of at most (d / 32 + 80) roundings each, some on the way of the other factor
+too; errors are measured against the largest magnitude of each result, of which sums of random terms stay a part: 2 * 7 * (d / 32 + 80)
+u = 1.1e-4 is the bound."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T,d,E,k,align", [(1, 64, 4, 2, 1), (203, 256, 8, 2, 16), (130, 128, 64, 6, 128)])
+def test_training_step(T, d, E, k, align):
+    from omega_ai_b200 import GradList, TokenSort, layer_norm, layer_norm_backward, native
+
+    L = native.lib()
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, dy = rn(T, d) + 0.5, rn(T, d)
+    gamma, beta, w_r, w_e = 1 + 0.1 * rn(d), 0.1 * rn(d), 0.05 * rn(E, d), rn(E, d, d) * d ** -0.5
+    idx, w = torch.empty(T, k, dtype=torch.int32, device="cuda"), torch.empty(T, k, device="cuda")
+    counts = torch.empty(E, dtype=torch.int32, device="cuda")
+
+    h, mean, rstd = layer_norm(x, gamma, beta, stats=True)
+    rc = L.omoe_route_noalloc(h.data_ptr(), w_r.data_ptr(), None, T, d, E, k, 1, native.OMOE_F32, idx.data_ptr(), w.data_ptr(),
+                              counts.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    sort = TokenSort(T, k, E, row_align=align).plan(idx)
+    assert torch.equal(sort.counts, counts)
+    xs = sort.sort(h)
+    start = sort.offsets.tolist()
+    ys = torch.zeros_like(xs)
+    for e in range(E):
+        ys[start[e]:start[e + 1]] = (xs[start[e]:start[e + 1]].double() @ w_e[e].double().T).float()
+    y = sort.unsort(ys, w)
+    # backward
+    dys, dw = sort.unsort_backward(dy, ys, w)
+    dxs, dwe = torch.zeros_like(xs), torch.zeros_like(w_e)
+    for e in range(E):
+        part = slice(start[e], start[e + 1])  # padding rows are zeros on both sides: whole segments go into the products
+        dxs[part] = (dys[part].double() @ w_e[e].double()).float()
+        dwe[e] = (dys[part].double().T @ xs[part].double()).float()
+    dh = sort.sort_backward(dxs)
+    dx, dgamma, dbeta = layer_norm_backward(dh, x, gamma, mean, rstd)
+    grads = [dwe, dgamma, dbeta]
+    unclipped = [t.clone() for t in grads]
+    norm = GradList(grads).clip(0.5)
+
+    X, G, B, W, WE = (t.double().requires_grad_() for t in (x, gamma, beta, w, w_e))
+    var, m = torch.var_mean(X, dim=1, correction=0, keepdim=True)
+    H = (X - m) / (var + 1e-5).sqrt() * G + B
+    Y = torch.zeros_like(H)
+    for j in range(k):
+        Y = Y + W[:, j:j + 1] * torch.einsum("tod,td->to", WE[idx[:, j].long()], H)
+    grads64 = torch.autograd.grad(Y, [X, G, B, W, WE], dy.double())
+    bound = 2 * 7 * (d / 32 + 80) * 2.0 ** -24
+    for got, want in zip((y, dx, unclipped[1], unclipped[2], dw, unclipped[0]), (Y.detach(), *grads64)):
+        assert (got.double() - want).abs().max() <= bound * want.abs().max()
+    norm64 = torch.stack([grads64[i].square().sum() for i in (4, 1, 2)]).sum().sqrt()
+    assert abs(float(norm) - float(norm64)) <= bound * float(norm64)
+    for got, want in zip(grads, (grads64[4], grads64[1], grads64[2])):
+        want = want * min(1.0, 0.5 / (float(norm64) + 1e-6))
+        assert (got.double() - want).abs().max() <= 3 * bound * want.abs().max()
+
+
+def test_norm_in_front_of_the_layer_and_its_gradients_clipped():
+    """LayerNorm -> MoELayer forward and backward -> LayerNorm backward, the layer's own gradients clipped with the norm's."""
+    from omega_ai_b200 import GradList, MoELayer, layer_norm, layer_norm_backward
+
+    T, d, dff, E, k = 96, 128, 256, 8, 2
+    layer = MoELayer(d, dff, E, k, t_max=T, compute_dtype=torch.bfloat16)
+    layer.initParam(seed=3)
+    layer.set_training(True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(T, d, generator=g, device="cuda") for _ in range(2))
+    gamma, beta = 1 + 0.1 * torch.randn(d, generator=g, device="cuda"), torch.zeros(d, device="cuda")
+    h, mean, rstd = layer_norm(x, gamma, beta, dtype=torch.bfloat16, stats=True)
+    y = layer.forward_device(h)
+    dh = layer.backward(h, dy.to(torch.bfloat16))
+    dx, dgamma, dbeta = layer_norm_backward(dh, x, gamma, mean, rstd)
+    grads = list(layer.weight_grads().values()) + [dgamma, dbeta]
+    ref = torch.stack([t.double().square().sum() for t in grads]).sum().sqrt()
+    before = [t.clone() for t in grads]
+    norm = GradList(grads).clip(0.01 * float(ref))
+    assert y.isfinite().all() and dx.isfinite().all()
+    assert abs(float(norm) - float(ref)) <= 5 * 2.0 ** -24 * float(ref)
+    after = torch.stack([t.double().square().sum() for t in grads]).sum().sqrt()
+    assert abs(float(after) / (0.01 * float(ref)) - 1) <= 1e-4
+    assert all(((a == 0) == (b == 0)).all() for a, b in zip(grads, before))
+    layer.close()
