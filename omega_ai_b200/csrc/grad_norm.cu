@@ -58,56 +58,66 @@ __device__ __forceinline__ double block_sum(double v, double *s) {
     return sum;
 }
 
-// The values of this thread in the chunk that starts at `p` with n elements; missing ones are 0.
+// The chunk's elements as this thread sees them.  Aligned chunks: vectors of 16 bytes, thread after thread, and what is left behind the
+// last whole vector one element per thread in `rest`.  Others: element by element.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T *p, int n, float (&v)[kPerThread]) {
-    constexpr int V = 16 / sizeof(T);
-    if (n == kChunkElems && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-        uint4 r[kPerThread / V];
+struct Chunk {
+    static constexpr int V = 16 / sizeof(T), N = kPerThread / V;
+    static __device__ __forceinline__ void unpack(const uint4 &r, float *v) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int i = 0; i < kPerThread / V; i++) r[i] = *(reinterpret_cast<const uint4 *>(p) + i * kThreads + threadIdx.x);
-#pragma unroll
-        for (int i = 0; i < kPerThread / V; i++) {
-            const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (V == 4) v[i * 4 + j] = __uint_as_float(w[j]);
-                else {
-                    v[i * 8 + 2 * j] = __uint_as_float(w[j] << 16);
-                    v[i * 8 + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                }
+        for (int j = 0; j < 4; j++) {
+            if constexpr (V == 4) v[j] = __uint_as_float(w[j]);
+            else {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
             }
         }
-    } else {
+    }
+    static __device__ __forceinline__ uint4 pack(const float *v) {
+        if constexpr (V == 4)
+            return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else
+            return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+    float v[kPerThread], rest;
+    __device__ __forceinline__ void load(const T *p, int n, bool vec) {
+        rest = 0.f;
+        if (vec) {
+            const int whole = n / V;
+            uint4 r[N];
 #pragma unroll
-        for (int i = 0; i < kPerThread; i++) {
-            const int at = i * kThreads + threadIdx.x;
-            v[i] = at < n ? (float)p[at] : 0.f;
+            for (int i = 0; i < N; i++) {
+                r[i] = make_uint4(0, 0, 0, 0);
+                if (i * kThreads + (int)threadIdx.x < whole) r[i] = *(reinterpret_cast<const uint4 *>(p) + i * kThreads + threadIdx.x);
+            }
+            if (whole * V + (int)threadIdx.x < n) rest = (float)p[whole * V + threadIdx.x];
+#pragma unroll
+            for (int i = 0; i < N; i++) unpack(r[i], v + i * V);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPerThread; i++) v[i] = i * kThreads + (int)threadIdx.x < n ? (float)p[i * kThreads + threadIdx.x] : 0.f;
         }
     }
-}
-
-template <typename T>
-__device__ __forceinline__ void scale_chunk(const T *p, T *o, int n, float c) {
-    constexpr int V = 16 / sizeof(T);
-    if (n == kChunkElems && ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15u) == 0) {
-        float v[kPerThread];
-        load_chunk(p, n, v);
+    __device__ __forceinline__ void scale(float c) {
 #pragma unroll
-        for (int i = 0; i < kPerThread / V; i++) {
-            uint4 r;
-            if constexpr (V == 4)
-                r = make_uint4(__float_as_uint(v[i * 4] * c), __float_as_uint(v[i * 4 + 1] * c), __float_as_uint(v[i * 4 + 2] * c),
-                               __float_as_uint(v[i * 4 + 3] * c));
-            else
-                r = make_uint4(pack_bf16(v[i * 8] * c, v[i * 8 + 1] * c), pack_bf16(v[i * 8 + 2] * c, v[i * 8 + 3] * c),
-                               pack_bf16(v[i * 8 + 4] * c, v[i * 8 + 5] * c), pack_bf16(v[i * 8 + 6] * c, v[i * 8 + 7] * c));
-            *(reinterpret_cast<uint4 *>(o) + i * kThreads + threadIdx.x) = r;
-        }
-    } else {
-        for (int at = threadIdx.x; at < n; at += kThreads) o[at] = (T)((float)p[at] * c);
+        for (int i = 0; i < kPerThread; i++) v[i] *= c;
+        rest *= c;
     }
-}
+    __device__ __forceinline__ void store(T *p, int n, bool vec) const {
+        if (vec) {
+            const int whole = n / V;
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i * kThreads + (int)threadIdx.x < whole) *(reinterpret_cast<uint4 *>(p) + i * kThreads + threadIdx.x) = pack(v + i * V);
+            if (whole * V + (int)threadIdx.x < n) p[whole * V + threadIdx.x] = (T)rest;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPerThread; i++)
+                if (i * kThreads + (int)threadIdx.x < n) p[i * kThreads + threadIdx.x] = (T)v[i];
+        }
+    }
+};
 
 // Calls f(entry, first element, elements) for every chunk of this block's part.
 template <int N, typename F>
@@ -137,10 +147,14 @@ grad_squares_kernel(const __grid_constant__ Table<N> t, double *__restrict__ slo
     pdl_wait();
     double sum = 0.0;
     walk(t, [&](const Entry &e, int64_t at, int n) {
-        float v[kPerThread];
-        if (e.dtype == OMOE_F32) load_chunk(static_cast<const float *>(e.in) + at, n, v);
-        else load_chunk(static_cast<const __nv_bfloat16 *>(e.in) + at, n, v);
-        sum += squares(v);
+        auto add = [&](auto *p) {
+            Chunk<std::remove_const_t<std::remove_pointer_t<decltype(p)>>> x;
+            x.load(p + at, n, (reinterpret_cast<uintptr_t>(p) & 15u) == 0);
+            sum += squares(x.v);
+            if (x.rest != 0.f) sum = fma((double)x.rest, (double)x.rest, sum);
+        };
+        if (e.dtype == OMOE_F32) add(static_cast<const float *>(e.in));
+        else add(static_cast<const __nv_bfloat16 *>(e.in));
     });
     sum = block_sum(sum, s);
     if (threadIdx.x == 0) slots[blockIdx.x] = add ? slots[blockIdx.x] + sum : sum;
@@ -176,9 +190,15 @@ grad_scale_kernel(const __grid_constant__ Table<N> t, const double *__restrict__
     if (norm < INFINITY) c = (float)fmin(1.0, (double)max_norm / ((double)norm + 1e-6));
     if (in_place && c == 1.f) return;
     walk(t, [&](const Entry &e, int64_t at, int n) {
-        if (e.dtype == OMOE_F32) scale_chunk(static_cast<const float *>(e.in) + at, static_cast<float *>(e.out) + at, n, c);
-        else
-            scale_chunk(static_cast<const __nv_bfloat16 *>(e.in) + at, static_cast<__nv_bfloat16 *>(e.out) + at, n, c);
+        auto scale = [&](auto *p, auto *o) {
+            Chunk<std::remove_pointer_t<decltype(o)>> x;
+            const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15u) == 0;
+            x.load(p + at, n, vec);
+            x.scale(c);
+            x.store(o + at, n, vec);
+        };
+        if (e.dtype == OMOE_F32) scale(static_cast<const float *>(e.in), static_cast<float *>(e.out));
+        else scale(static_cast<const __nv_bfloat16 *>(e.in), static_cast<__nv_bfloat16 *>(e.out));
     });
 }
 

@@ -62,6 +62,10 @@ struct Frag<float, 8> {
         a = __ldcs(reinterpret_cast<const float4 *>(p));
         b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
     }
+    __device__ __forceinline__ void load_cached(const float *p) {
+        a = __ldg(reinterpret_cast<const float4 *>(p));
+        b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    }
     __device__ __forceinline__ void store(float *p) const {
         *reinterpret_cast<float4 *>(p) = a;
         *(reinterpret_cast<float4 *>(p) + 1) = b;
@@ -79,6 +83,7 @@ template <>
 struct Frag<float, 1> {
     float r;
     __device__ __forceinline__ void load(const float *p) { r = __ldcs(p); }
+    __device__ __forceinline__ void load_cached(const float *p) { r = __ldg(p); }
     __device__ __forceinline__ void store(float *p) const { *p = r; }
     __device__ __forceinline__ void zero() { r = 0.f; }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = r; }

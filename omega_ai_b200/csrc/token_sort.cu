@@ -19,9 +19,10 @@ constexpr int kPlanBatch = 8;    // picks a lane loads together
 constexpr int kPlanCtasMax = 8;  // the portable cluster size
 
 // One cluster does the whole plan.  Every warp owns a contiguous run of picks and counts its picks of every expert in
-// shared memory (lanes with the same expert are found with a match, the lowest adds them up); after sums over the
-// warps and, through distributed shared memory, over the CTAs every warp knows where its first pick of each
-// expert goes, walks its run again and numbers the picks.  Bound by latency: the two walks and the barriers.
+// shared memory, numbering them as it goes: lanes with the same expert are found by ballots over the bits of its number (a warp-wide
+// match takes longer the more experts meet in a warp).  After sums over the warps and, through distributed shared memory,
+// over the CTAs every warp knows where its first pick of each expert goes.  A run of up to 256 picks stays in
+// registers, a longer one keeps its numbers in pos meanwhile.  Bound by latency: the walk and the barriers.
 __global__ void __launch_bounds__(kPlanWarps * 32)
 sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int rows_cap, int warp_run,
                  int32_t *__restrict__ pos, int32_t *__restrict__ perm, int32_t *__restrict__ counts,
@@ -42,23 +43,31 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     const int lo = (int)min((int64_t)n, lo64), hi = (int)min((int64_t)n, lo64 + warp_run);
     pdl_wait();
     __syncwarp();
-    int32_t key[kPlanBatch];
-    auto fetch = [&](int i0) {
+    const int bits = 32 - __clz(E);  // of the keys 0..E, E standing for no expert
+    int32_t key[kPlanBatch], rank[kPlanBatch];
+    for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
 #pragma unroll
         for (int u = 0; u < kPlanBatch; u++) {
             const int i = i0 + u * 32 + lane;
             const int e = i < hi ? idx[i] : -1;
-            key[u] = e >= 0 && e < E ? e : -1;
+            key[u] = e >= 0 && e < E ? e : E;
         }
-    };
-    for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
-        fetch(i0);
 #pragma unroll
         for (int u = 0; u < kPlanBatch; u++) {
+            const int i = i0 + u * 32 + lane;
             if (i0 + u * 32 >= hi) break;
-            const uint32_t same = __match_any_sync(0xffffffffu, key[u]);
-            if (key[u] >= 0 && lane == __ffs(same) - 1) hist[key[u]] += __popc(same);
+            uint32_t same = 0xffffffffu;  // lanes with this lane's key
+            for (int b = 0; b < bits; b++) {
+                const uint32_t set = __ballot_sync(0xffffffffu, (key[u] >> b) & 1);
+                same &= (key[u] >> b) & 1 ? set : ~set;
+            }
+            const uint32_t before = same & ((1u << lane) - 1);
+            rank[u] = 0;
+            if (key[u] < E) rank[u] = hist[key[u]] + __popc(before);
             __syncwarp();
+            if (key[u] < E && !before) hist[key[u]] += __popc(same);
+            __syncwarp();
+            if (warp_run > kPlanBatch * 32 && i < hi) pos[i] = rank[u];  // kept there until the expert's first row is known
         }
     }
     __syncthreads();
@@ -117,21 +126,22 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     __syncthreads();
     for (int64_t r = (int64_t)s_start[E] + cta * blockDim.x + threadIdx.x; r < rows_cap; r += ctas * blockDim.x) perm[r] = -1;
     for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
-        if (warp_run > kPlanBatch * 32) fetch(i0);
+        if (warp_run > kPlanBatch * 32) {
+#pragma unroll
+            for (int u = 0; u < kPlanBatch; u++) {
+                const int i = i0 + u * 32 + lane;
+                key[u] = i < hi ? idx[i] : -1;
+                rank[u] = i < hi ? pos[i] : 0;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < kPlanBatch; u++) {
-            const int i = i0 + u * 32 + lane, e = key[u];
-            if (i0 + u * 32 >= hi) break;
-            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int i = i0 + u * 32 + lane;
+            if (i >= hi) continue;
             int row = -1;
-            if (e >= 0) row = s_start[e] + hist[e] + __popc(same & ((1u << lane) - 1));
-            __syncwarp();
-            if (e >= 0 && lane == __ffs(same) - 1) hist[e] += __popc(same);
-            __syncwarp();
-            if (i < hi) {
-                pos[i] = row;
-                if (row >= 0 && row < rows_cap) perm[row] = i;
-            }
+            if (key[u] >= 0 && key[u] < E) row = s_start[key[u]] + hist[key[u]] + rank[u];
+            pos[i] = row;
+            if (row >= 0 && row < rows_cap) perm[row] = i;
         }
     }
     if (ctas > 1) cluster.sync();  // the others may still read this CTA's totals
@@ -148,23 +158,34 @@ __device__ __forceinline__ int pick_row(const int32_t *pos, int64_t t, int k, in
     return r < rows_cap ? r : -1;
 }
 
-// Zeros for the padding rows of expert e, columns [c0, c1), by one warp.
+// Padding rows of an expert are zeroed by kPadRows at a time, each slice by a warp or block of its own: one warp for all of an
+// expert's up to 127 rows took longer than the whole copy.
+constexpr int kPadRows = 8, kPadSlicesMax = 128;
+int pad_slices(int align) {
+    const int n = (align - 1 + kPadRows - 1) / kPadRows;
+    return n < kPadSlicesMax ? n : kPadSlicesMax;
+}
+
+// Zeros for the padding rows of slice `item` (experts times slices), columns c0, c0 + step, ... below c1.
 template <typename T, int V>
-__device__ __forceinline__ void zero_padding(T *rows, int64_t ld, const int32_t *counts, const int32_t *offsets, int e, int c0,
-                                             int c1, int lane, int rows_cap) {
-    const int first = offsets[e] + counts[e], last = min(offsets[e + 1], rows_cap);
+__device__ __forceinline__ void zero_padding(T *rows, int64_t ld, const int32_t *counts, const int32_t *offsets, int item, int slices,
+                                             int c0, int c1, int step, int rows_cap) {
+    const int e = item / slices, first = offsets[e] + counts[e], last = min(offsets[e + 1], rows_cap);
+    if (first < 0) return;
     Frag<T, V> z;
     z.zero();
-    if (first < 0) return;
-    for (int r = first; r < last; r++)
-        for (int c = c0 + lane * V; c < c1; c += 32 * V) z.store(rows + (int64_t)r * ld + c);
+    for (int r0 = first + item % slices * kPadRows; r0 < last; r0 += slices * kPadRows)
+        for (int c = c0; c < c1; c += step)
+#pragma unroll
+            for (int r = 0; r < kPadRows; r++)
+                if (r0 + r < last) z.store(rows + (int64_t)(r0 + r) * ld + c);
 }
 
 // xs[pos] = x: a warp reads a chunk of a token's row once and stores it for every pick.  HBM bound.
 template <typename XT, typename OT, int V>
 __global__ void __launch_bounds__(256)
 sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int64_t ldxs, const int32_t *__restrict__ pos,
-                 const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int T, int k, int E, int d,
+                 const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int T, int k, int pads, int slices, int d,
                  int n_chunks, int rows_cap) {
     constexpr int U = kChunk<V> / (32 * V);
     const int lane = threadIdx.x & 31;
@@ -174,7 +195,8 @@ sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int
     pdl_trigger();
     pdl_wait();
     if (t >= T) {
-        if (t - T < E) zero_padding<OT, V>(xs, ldxs, counts, offsets, (int)(t - T), c0 - lane * V, min(d, c0 - lane * V + kChunk<V>), lane, rows_cap);
+        if (t - T < pads)
+            zero_padding<OT, V>(xs, ldxs, counts, offsets, (int)(t - T), slices, c0, min(d, c0 - lane * V + kChunk<V>), 32 * V, rows_cap);
         return;
     }
     const int r = pick_row(pos, t, k, lane, rows_cap);
@@ -262,16 +284,15 @@ template <typename DT, typename YT, int V, int K>
 __global__ void __launch_bounds__(512)
 unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict__ ys, int64_t ldys, YT *__restrict__ dys,
                   int64_t lddys, const int32_t *__restrict__ pos, const int32_t *__restrict__ counts,
-                  const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int E,
+                  const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int slices,
                   int d, int rows_cap) {
     __shared__ float s_dot[16][K];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
     const int64_t t = blockIdx.x;
     pdl_trigger();
     pdl_wait();
-    if (t >= T) {  // a block per expert for its padding rows, a warp per part of the columns
-        const int part = ((d + nw - 1) / nw + V * 32 - 1) / (V * 32) * (V * 32), c0 = warp * part;
-        if (c0 < d) zero_padding<YT, V>(dys, lddys, counts, offsets, (int)(t - T), c0, min(d, c0 + part), lane, rows_cap);
+    if (t >= T) {
+        zero_padding<YT, V>(dys, lddys, counts, offsets, (int)(t - T), slices, threadIdx.x * V, d, blockDim.x * V, rows_cap);
         return;
     }
     int row[K];
@@ -416,7 +437,8 @@ int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_
     if (int rc = check_rows(all, 2, 1, fn)) return rc;
     if (T == 0) return ops_ok();
     const bool vec = rows_vector(x) && rows_vector(xs);
-    const int64_t tokens = T + (plan->row_align > 1 ? E : 0);  // an expert's padding is one more "token"
+    const int slices = pad_slices(plan->row_align), pads = E * slices;
+    const int64_t tokens = (int64_t)T + pads;  // a slice of an expert's padding is one more "token"
     const int64_t blocks = ((vec ? row_items<8>(tokens, d) : row_items<1>(tokens, d)) + 7) / 8;
     if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
     return ops_launched(by_types(x_dtype, xs_dtype, [&](auto *xt, auto *ot) {
@@ -425,7 +447,7 @@ int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_
         auto go = [&](auto kern, int chunk) {
             return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
                              static_cast<const XT *>(x_dev), ldx, static_cast<OT *>(xs_dev), ldxs, plan->pos, plan->counts,
-                             plan->offsets, T, plan->top_k, E, d, ceil_div(d, chunk), (int)plan->rows_cap);
+                             plan->offsets, T, plan->top_k, pads, slices, d, ceil_div(d, chunk), (int)plan->rows_cap);
         };
         return vec ? go(sort_rows_kernel<XT, OT, 8>, kChunk<8>) : go(sort_rows_kernel<XT, OT, 1>, kChunk<1>);
     }), fn);
@@ -478,7 +500,8 @@ int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t
     if (int rc = check_rows(all, dw_dev ? 3 : 2, 1, fn)) return rc;
     if (misaligned(w_dev, 4) || misaligned(dw_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
     if (T == 0) return ops_ok();
-    const int64_t blocks = (int64_t)T + (plan->row_align > 1 ? E : 0);
+    const int slices = pad_slices(plan->row_align);
+    const int64_t blocks = (int64_t)T + E * slices;
     if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
     const bool vec = rows_vector(dys) && rows_vector(dy) && (!dw_dev || rows_vector(ys));
     const int per = vec ? 8 : 1;
@@ -490,7 +513,7 @@ int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t
         auto go = [&](auto kern) {
             return launch_ex(kern, dim3((unsigned)blocks), dim3(threads), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
                              static_cast<const DT *>(dy_dev), lddy, static_cast<const YT *>(ys_dev), ldys,
-                             static_cast<YT *>(dys_dev), lddys, plan->pos, plan->counts, plan->offsets, w_dev, dw_dev, T, k, E,
+                             static_cast<YT *>(dys_dev), lddys, plan->pos, plan->counts, plan->offsets, w_dev, dw_dev, T, k, slices,
                              d, (int)plan->rows_cap);
         };
         auto by_k = [&](auto v) {

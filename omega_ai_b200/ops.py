@@ -16,54 +16,49 @@ from .layer import Layer, Tensor, _dt
 from .native import OmoeError
 
 
-def _check(rc: int):
-    if rc != 0:
-        raise OmoeError(rc, native.lib().omoe_ops_error().decode())
-
-
 def _bad(message: str):
     raise OmoeError(-1, message)
 
 
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream() takes 3 us to say the same
+
+
+def _call(device, f, *args):
+    """The entry point f on the device's current stream, with that device current."""
+    index = device.index
+    if device.type != "cuda":
+        _bad(f"tensors must be on a GPU, got {device}")
+    if _current_device() == index:
+        rc = f(*args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _current_stream(index))
+    if rc != 0:
+        raise OmoeError(rc, native.lib().omoe_ops_error().decode())
+
+
 def _matrix(t: torch.Tensor, rows: int, d: int, name: str, device) -> int:
     """Leading dimension of a [rows, d] matrix on ``device``."""
-    if t.device != device or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != d:
+    if t.shape != (rows, d) or t.device != device:
         _bad(f"{name}: expected [{rows}, {d}] on {device}, got {list(t.shape)} on {t.device}")
-    if d > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if one != 1 and d > 1:
         _bad(f"{name}: the elements of a row must be contiguous")
     if rows <= 1:
         return d
-    if t.stride(0) < d:
+    if ld < d:
         _bad(f"{name}: rows overlap")
-    return t.stride(0)
+    return ld
 
 
 def _vector(t, n: int, name: str, device, dtype=torch.float32):
     """Address of a contiguous buffer of n elements, None for None."""
     if t is None:
         return None
-    if t.device != device or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
         _bad(f"{name}: expected {n} contiguous {dtype} on {device}")
     return t.data_ptr()
-
-
-class _on:
-    """The stream to enqueue on, with the tensors' device current for the duration of the call."""
-
-    def __init__(self, device):
-        if device.type != "cuda":
-            _bad(f"tensors must be on a GPU, got {device}")
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
 
 
 class TokenSort:
@@ -94,8 +89,7 @@ class TokenSort:
     def plan(self, topk_idx: torch.Tensor) -> "TokenSort":
         """From the picks [T, k], int32, as the routing leaves them."""
         at = _vector(topk_idx, self.tokens * self.top_k, "topk_idx", self.device, torch.int32)
-        with _on(self.device) as s:
-            _check(self._lib.omoe_sort_plan(self._p, at, s))
+        _call(self.device, self._lib.omoe_sort_plan, self._p, at)
         return self
 
     def _out(self, out, rows, d, dtype, name):
@@ -107,19 +101,18 @@ class TokenSort:
         """xs[pos[t, j]] = x[t]; padding rows zero, rows behind the last expert's as they were."""
         d = x.shape[-1]
         ldx = _matrix(x, self.tokens, d, "x", self.device)
-        with _on(self.device) as s:
-            out, ldo = self._out(out, self.rows_cap, d, dtype or x.dtype, "out")
-            _check(self._lib.omoe_sort_rows(self._p, x.data_ptr(), ldx, _dt(x.dtype), out.data_ptr(), ldo, _dt(out.dtype), d, s))
+        out, ldo = self._out(out, self.rows_cap, d, dtype or x.dtype, "out")
+        _call(self.device, self._lib.omoe_sort_rows, self._p, x.data_ptr(), ldx, _dt(x.dtype), out.data_ptr(), ldo,
+              _dt(out.dtype), d)
         return out
 
     def sort_backward(self, dxs: torch.Tensor, out=None, dtype=None) -> torch.Tensor:
         """dx[t] = sum over the token's picks of dxs[pos[t, j]]."""
         d = dxs.shape[-1]
         ldx = _matrix(dxs, self.rows_cap, d, "dxs", self.device)
-        with _on(self.device) as s:
-            out, ldo = self._out(out, self.tokens, d, dtype or dxs.dtype, "out")
-            _check(self._lib.omoe_sort_rows_backward(self._p, dxs.data_ptr(), ldx, _dt(dxs.dtype), out.data_ptr(), ldo,
-                                                     _dt(out.dtype), d, s))
+        out, ldo = self._out(out, self.tokens, d, dtype or dxs.dtype, "out")
+        _call(self.device, self._lib.omoe_sort_rows_backward, self._p, dxs.data_ptr(), ldx, _dt(dxs.dtype), out.data_ptr(),
+              ldo, _dt(out.dtype), d)
         return out
 
     def unsort(self, ys: torch.Tensor, weights=None, out=None, dtype=None) -> torch.Tensor:
@@ -127,10 +120,9 @@ class TokenSort:
         d = ys.shape[-1]
         ldy = _matrix(ys, self.rows_cap, d, "ys", self.device)
         w = _vector(weights, self.tokens * self.top_k, "weights", self.device)
-        with _on(self.device) as s:
-            out, ldo = self._out(out, self.tokens, d, dtype or ys.dtype, "out")
-            _check(self._lib.omoe_unsort_rows(self._p, ys.data_ptr(), ldy, _dt(ys.dtype), w, out.data_ptr(), ldo,
-                                              _dt(out.dtype), d, s))
+        out, ldo = self._out(out, self.tokens, d, dtype or ys.dtype, "out")
+        _call(self.device, self._lib.omoe_unsort_rows, self._p, ys.data_ptr(), ldy, _dt(ys.dtype), w, out.data_ptr(), ldo,
+              _dt(out.dtype), d)
         return out
 
     def unsort_backward(self, dy: torch.Tensor, ys: torch.Tensor, weights=None, out=None):
@@ -140,14 +132,12 @@ class TokenSort:
         lddy = _matrix(dy, self.tokens, d, "dy", self.device)
         ldys = _matrix(ys, self.rows_cap, d, "ys", self.device)
         w = _vector(weights, self.tokens * self.top_k, "weights", self.device)
-        with _on(self.device) as s:
-            out, ldo = self._out(out, self.rows_cap, d, ys.dtype, "out")
-            if out.dtype != ys.dtype:
-                _bad("out: must have the type of ys")
-            dw = None if weights is None else torch.empty(self.tokens, self.top_k, dtype=torch.float32, device=self.device)
-            _check(self._lib.omoe_unsort_rows_backward(
-                self._p, dy.data_ptr(), lddy, _dt(dy.dtype), ys.data_ptr(), ldys, _dt(ys.dtype), w, out.data_ptr(), ldo,
-                None if dw is None else dw.data_ptr(), d, s))
+        out, ldo = self._out(out, self.rows_cap, d, ys.dtype, "out")
+        if out.dtype != ys.dtype:
+            _bad("out: must have the type of ys")
+        dw = None if weights is None else torch.empty(self.tokens, self.top_k, dtype=torch.float32, device=self.device)
+        _call(self.device, self._lib.omoe_unsort_rows_backward, self._p, dy.data_ptr(), lddy, _dt(dy.dtype), ys.data_ptr(),
+              ldys, _dt(ys.dtype), w, out.data_ptr(), ldo, None if dw is None else dw.data_ptr(), d)
         return out, dw
 
 
@@ -158,16 +148,16 @@ def layer_norm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=No
         _bad(f"x: expected [T, d], got {list(x.shape)}")
     T, d = x.shape
     dev = x.device
-    with _on(dev) as s:
-        ldx = _matrix(x, T, d, "x", dev)
-        if out is None:
-            out = torch.empty(T, d, dtype=dtype or x.dtype, device=dev)
-        ldo = _matrix(out, T, d, "out", dev)
-        mean = torch.empty(T, dtype=torch.float32, device=dev) if stats else None
-        rstd = torch.empty_like(mean) if stats else None
-        _check(native.lib().omoe_layer_norm(
-            x.data_ptr(), ldx, _dt(x.dtype), _vector(gamma, d, "gamma", dev), _vector(beta, d, "beta", dev), eps,
-            out.data_ptr(), ldo, _dt(out.dtype), mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, T, d, s))
+    ldx = _matrix(x, T, d, "x", dev)
+    if out is None:
+        out = torch.empty(T, d, dtype=dtype or x.dtype, device=dev)
+    ldo = _matrix(out, T, d, "out", dev)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty(T, dtype=torch.float32, device=dev), torch.empty(T, dtype=torch.float32, device=dev)
+    _call(dev, native.lib().omoe_layer_norm, x.data_ptr(), ldx, _dt(x.dtype), _vector(gamma, d, "gamma", dev),
+          _vector(beta, d, "beta", dev), eps, out.data_ptr(), ldo, _dt(out.dtype), mean.data_ptr() if stats else None,
+          rstd.data_ptr() if stats else None, T, d)
     return (out, mean, rstd) if stats else out
 
 
@@ -179,23 +169,22 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma, mean: torch.Te
     T, d = x.shape
     dev = x.device
     L = native.lib()
-    with _on(dev) as s:
-        ldx, lddy = _matrix(x, T, d, "x", dev), _matrix(dy, T, d, "dy", dev)
-        if out is None:
-            out = torch.empty(T, d, dtype=x.dtype, device=dev)
-        ldo = _matrix(out, T, d, "out", dev)
-        if out.dtype != x.dtype:
-            _bad("out: must have the type of x")
-        if d == 0:
-            _bad("x: no columns")
-        dgamma = torch.empty(d, dtype=torch.float32, device=dev) if param_grads else None
-        dbeta = torch.empty_like(dgamma) if param_grads else None
-        ws = torch.empty(L.omoe_layer_norm_backward_workspace(T, d), dtype=torch.uint8, device=dev)
-        _check(L.omoe_layer_norm_backward(
-            dy.data_ptr(), lddy, _dt(dy.dtype), x.data_ptr(), ldx, _dt(x.dtype), _vector(gamma, d, "gamma", dev),
-            _vector(mean, T, "mean", dev), _vector(rstd, T, "rstd", dev), out.data_ptr(), ldo,
-            dgamma.data_ptr() if param_grads else None, dbeta.data_ptr() if param_grads else None, T, d, ws.data_ptr(),
-            ws.numel(), s))
+    ldx, lddy = _matrix(x, T, d, "x", dev), _matrix(dy, T, d, "dy", dev)
+    if out is None:
+        out = torch.empty(T, d, dtype=x.dtype, device=dev)
+    ldo = _matrix(out, T, d, "out", dev)
+    if out.dtype != x.dtype:
+        _bad("out: must have the type of x")
+    if d == 0:
+        _bad("x: no columns")
+    dgamma = dbeta = None
+    if param_grads:
+        dgamma, dbeta = torch.empty(2, d, dtype=torch.float32, device=dev)
+    size = L.omoe_layer_norm_backward_workspace(T, d)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _call(dev, L.omoe_layer_norm_backward, dy.data_ptr(), lddy, _dt(dy.dtype), x.data_ptr(), ldx, _dt(x.dtype),
+          _vector(gamma, d, "gamma", dev), _vector(mean, T, "mean", dev), _vector(rstd, T, "rstd", dev), out.data_ptr(), ldo,
+          dgamma.data_ptr() if param_grads else None, dbeta.data_ptr() if param_grads else None, T, d, ws.data_ptr(), size)
     return out, dgamma, dbeta
 
 
@@ -250,19 +239,19 @@ class GradList:
 
     def norm(self) -> torch.Tensor:
         """The norm of all elements, fp32 on the device."""
-        with _on(self.device) as s:
-            norm, ws = self._new()
-            _check(self._lib.omoe_grad_norm(self._in, len(self.grads), norm.data_ptr(), ws.data_ptr(), ws.numel(), s))
+        norm, ws = self._new()
+        _call(self.device, self._lib.omoe_grad_norm, self._in, len(self.grads), norm.data_ptr(), ws.data_ptr(),
+              native.GRAD_WORKSPACE_BYTES)
         return norm
 
     def scale(self, norm: torch.Tensor, max_norm: float) -> None:
         """Times min(1, max_norm / (norm + 1e-6)), for a norm that covers more than this list; 1 where it is not finite."""
-        with _on(self.device) as s:
-            _check(self._lib.omoe_grad_scale(self._in, self._to, len(self.grads), _vector(norm, 1, "norm", self.device), max_norm, s))
+        _call(self.device, self._lib.omoe_grad_scale, self._in, self._to, len(self.grads),
+              _vector(norm, 1, "norm", self.device), max_norm)
 
     def clip(self, max_norm: float) -> torch.Tensor:
         """:meth:`norm` and :meth:`scale` in one; returns the norm before clipping."""
-        with _on(self.device) as s:
-            norm, ws = self._new()
-            _check(self._lib.omoe_grad_clip(self._in, self._to, len(self.grads), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), s))
+        norm, ws = self._new()
+        _call(self.device, self._lib.omoe_grad_clip, self._in, self._to, len(self.grads), max_norm, norm.data_ptr(),
+              ws.data_ptr(), native.GRAD_WORKSPACE_BYTES)
         return norm
