@@ -346,8 +346,8 @@ OMOE_API const char *omoe_route_noalloc_error(void);
  * thread's next call of one of these entry points.
  *
  * Rows are row-major with a leading dimension (elements from one row to the next, at least d).  Any width,
- * leading dimension and element-aligned address is taken; rows whose width is a multiple of 8 and whose address
- * and leading dimension keep every row 16-byte aligned move as vectors, others element by element.
+ * leading dimension and element-aligned address is taken; rows whose width and leading dimension are multiples of
+ * 8, at an address aligned to 8 elements, move as vectors, others element by element.
  */
 OMOE_API const char *omoe_ops_error(void);
 
@@ -408,7 +408,7 @@ OMOE_API int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev
  * omoe_layer_norm_backward: with g = dy * gamma and h = (x - mean) * rstd,
  *   dx = rstd * (g - mean(g) - h * mean(g * h)) of x's element type, dgamma = sum over the rows of dy * h,
  *   dbeta = sum over the rows of dy, fp32, overwritten.  dgamma and dbeta may be NULL.  workspace_dev holds at least
- * omoe_layer_norm_backward_workspace(T, d) bytes, 16-byte aligned, whose contents do not matter.
+ * omoe_layer_norm_backward_workspace(T, d) bytes, 32-byte aligned, whose contents do not matter.
  */
 OMOE_API int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float *gamma_dev,
                              const float *beta_dev, float eps, void *y_dev, int64_t ldy, int32_t y_dtype,

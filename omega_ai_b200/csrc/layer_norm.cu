@@ -12,6 +12,7 @@ namespace omoe {
 
 namespace {
 
+constexpr int kRowsMax = 0x7fff0000;  // row numbers, and the rows a grid takes at a time beyond them, fit 32 bits
 constexpr int kWideThreads = 512;
 
 // Sum over a block of kWideThreads, the same value in every thread.
@@ -45,7 +46,7 @@ norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict_
         const float v = (float)row[c] - mean;
         sum = fmaf(v, v, sum);
     }
-    const float rstd = 1.f / sqrtf(block_sum(sum, s) / (float)d + eps);
+    const float rstd = rsqrtf(block_sum(sum, s) / (float)d + eps);
     if (threadIdx.x == 0) {
         if (mean_out) mean_out[t] = mean;
         if (rstd_out) rstd_out[t] = rstd;
@@ -111,80 +112,187 @@ norm_cols_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__
 // ---- rows that fit a block's registers ----------------------------------------------------------------------------
 //
 // A block of 512 threads works on 512 / G rows at a time: G threads hold a row, P vectors of V elements each, and walk
-// the rows of the grid with a stride.  Rows arrive in a ring of S stages in shared memory by asynchronous copies; a thread
-// copies exactly the vectors it will read, so the ring needs no barrier, and the loads of the next S - 1 rows are on
-// their way while a row is reduced.  The reductions are what threads of a row meet for: warp shuffles, then one named barrier each.
+// the rows of the grid with a stride.  Rows arrive in a ring of S stages in shared memory by asynchronous copies that a warp makes for
+// its own columns alone, so the ring needs no block barrier, and the loads of the next S - 1 rows are on their way while a
+// row is reduced.  The reductions are what threads of a row meet for: warp shuffles, then one named barrier each.
+// Bound by the issue of instructions before it is by HBM, hence pairs of values in the packed fp32 instructions, sums that
+// share their shuffles, and no divisions.
 constexpr int kBlock = 512;
+
+// Two fp32 values in one register pair.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(b));
+    return a;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(b));
+    return a;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a) : "l"(b), "l"(c));
+    return a;
+}
+__device__ __forceinline__ float both(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return a + b;
+}
 
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last N groups of this warp's copies have landed, and its lanes are done with the stage they read before.
 template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
+}
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+    return r;
+}
 
-// This thread's vectors of the rows ahead.  V = 8: S stages of shared memory.  V = 1 (rows that are not 16-byte aligned):
-// one row ahead, in registers.
-template <typename T, int V, int P, int S>
+// The rows ahead.  V = 8: S stages of shared memory; a stage holds, for every vector of a thread, a plane of 16 bytes per
+// thread (two for fp32).  fp32 is copied by the lanes of a warp in the order of the addresses, not of the owners: 16 of the
+// owner's 32 bytes at a time would move every sector twice.
+// V = 1 (rows that are not aligned): one row ahead, in registers.
+template <typename T, int V, int G, int P, int S>
 struct Ahead {
-    uint32_t slot;
-    static constexpr int kBytes = V * sizeof(T);
+    static constexpr int kPlanes = sizeof(T) / 2;
+    static constexpr int kStage = kBlock * 16 * kPlanes * P;
+    uint32_t own, put;  // this thread's slot, and where it puts what it copies
+    int col;            // the first column it copies
     // vectors behind the row's end are zeros in every stage from the start
-    __device__ __forceinline__ Ahead(uint32_t ring, const int (&c)[P], int d) : slot(ring + threadIdx.x * 16) {
+    __device__ __forceinline__ Ahead(uint32_t ring, int d) {
+        const int lane = threadIdx.x & 31, in_row = threadIdx.x % G;
+        own = ring + threadIdx.x * 16;
+        put = kPlanes == 1 ? own : ring + (lane & 1) * (kBlock * 16) + (threadIdx.x - (lane + 1) / 2) * 16;
+        col = kPlanes == 1 ? in_row * 8 : (in_row - lane) * 8 + lane * 4;
 #pragma unroll
         for (int p = 0; p < P; p++)
-            if (c[p] >= d)
+            if ((p * G + in_row) * 8 >= d)
                 for (int i = 0; i < S; i++)
 #pragma unroll
-                    for (int q = 0; q < kBytes / 16; q++)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(slot + ((i * P + p) * (kBytes / 16) + q) * (kBlock * 16)), "r"(0) : "memory");
+                    for (int q = 0; q < kPlanes; q++)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(own + i * kStage + (p * kPlanes + q) * (kBlock * 16)), "r"(0) : "memory");
+        __syncwarp();
     }
-    static constexpr int kStage = kBlock * P * kBytes;
-    __device__ __forceinline__ void fetch(int stage, const T *row, const int (&c)[P], int d) {
+    __device__ __forceinline__ void fetch(int stage, const T *row, int d) const {
 #pragma unroll
         for (int p = 0; p < P; p++)
-            if (c[p] < d)
 #pragma unroll
-                for (int q = 0; q < kBytes / 16; q++)
-                    copy16(slot + ((stage * P + p) * (kBytes / 16) + q) * (kBlock * 16), reinterpret_cast<const char *>(row + c[p]) + q * 16);
-    }
-    __device__ __forceinline__ void take(int stage, float (&v)[P][V]) const {
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-            uint4 r[kBytes / 16];
-#pragma unroll
-            for (int q = 0; q < kBytes / 16; q++)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[q].x), "=r"(r[q].y), "=r"(r[q].z), "=r"(r[q].w)
-                             : "r"(slot + ((stage * P + p) * (kBytes / 16) + q) * (kBlock * 16)) : "memory");
-            if constexpr (sizeof(T) == 2) unpack8(r[0], v[p]);
-            else {
-                const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[p][i] = __uint_as_float(w[i]);
+            for (int q = 0; q < kPlanes; q++) {
+                const int c = col + p * G * 8 + q * 128;
+                if (c < d) copy16(put + stage * kStage + p * kPlanes * (kBlock * 16) + q * 256, row + c);
             }
+    }
+    // pairs 4p .. 4p + 3 of this thread
+    __device__ __forceinline__ void take(int stage, int p, f2 (&v)[4]) const {
+        const uint4 a = shared16(own + stage * kStage + p * kPlanes * (kBlock * 16));
+        if constexpr (kPlanes == 1) {
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        } else {
+            const uint4 b = shared16(own + stage * kStage + (p * kPlanes + 1) * (kBlock * 16));
+            v[0] = pack2(__uint_as_float(a.x), __uint_as_float(a.y));
+            v[1] = pack2(__uint_as_float(a.z), __uint_as_float(a.w));
+            v[2] = pack2(__uint_as_float(b.x), __uint_as_float(b.y));
+            v[3] = pack2(__uint_as_float(b.z), __uint_as_float(b.w));
         }
     }
 };
-template <typename T, int P, int S>
-struct Ahead<T, 1, P, S> {
+template <typename T, int G, int P, int S>
+struct Ahead<T, 1, G, P, S> {
+    static constexpr int kStage = 0;
     Frag<T, 1> next[P];
-    __device__ __forceinline__ Ahead(uint32_t, const int (&)[P], int) {
+    __device__ __forceinline__ Ahead(uint32_t, int) {
 #pragma unroll
         for (int p = 0; p < P; p++) next[p].zero();
     }
-    static constexpr int kStage = 0;
-    __device__ __forceinline__ void fetch(int, const T *row, const int (&c)[P], int d) {
+    __device__ __forceinline__ void fetch(int, const T *row, int d) {
 #pragma unroll
         for (int p = 0; p < P; p++)
-            if (c[p] < d) next[p].load(row + c[p]);
+            if (p * G + (int)(threadIdx.x % G) < d) next[p].load(row + p * G + threadIdx.x % G);
     }
-    __device__ __forceinline__ void take(int, float (&v)[P][1]) const {
+    // all of this thread's elements, two by two
+    __device__ __forceinline__ void take(int, int p, f2 (&v)[P / 2]) const {
 #pragma unroll
-        for (int p = 0; p < P; p++) next[p].get(v[p]);
+        for (int i = 0; i < P / 2; i++) {
+            float a[1], b[1];
+            next[2 * i].get(a);
+            next[2 * i + 1].get(b);
+            v[i] = pack2(a[0], b[0]);
+        }
     }
 };
 
-// Stages that fit a block's share of shared memory, where BLOCKS of them share an SM.
+// What a thread holds of a row, in groups of pairs that are read and stored together: a vector each (V = 8), or all of its
+// single elements (V = 1).
+template <int V, int G, int P>
+struct Part {
+    static constexpr int kGroups = V == 8 ? P : 1, kPairs = V == 8 ? 4 : P / 2;
+    int d;
+    __device__ __forceinline__ int in_row() const { return threadIdx.x % G; }
+    __device__ __forceinline__ int col(int q) const { return V == 8 ? (q * G + in_row()) * 8 : in_row(); }
+    __device__ __forceinline__ bool has(int q) const { return col(q) < d; }
+    // zeros in place of what lies behind the row's end
+    __device__ __forceinline__ void mask(int q, f2 (&v)[kPairs]) const {
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) {
+            if constexpr (V == 8) v[i] = has(q) ? v[i] : 0ull;
+            else {
+                float a, b;
+                unpack2(v[i], a, b);
+                v[i] = pack2(in_row() + 2 * i * G < d ? a : 0.f, in_row() + (2 * i + 1) * G < d ? b : 0.f);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const float *p, int q, float missing, f2 (&v)[kPairs]) const {
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) v[i] = pack2(missing, missing);
+        if (!p || !has(q)) return;
+        if constexpr (V == 8) {
+            Frag<float, 8> f;
+            f.load_cached(p + col(q));
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = pack2(f.r[2 * i], f.r[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; i++) {
+                const int a = in_row() + 2 * i * G, b = a + G;
+                v[i] = pack2(a < d ? __ldg(p + a) : missing, b < d ? __ldg(p + b) : missing);
+            }
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T *p, int q, const f2 (&v)[kPairs]) const {
+        float w[2 * kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) unpack2(v[i], w[2 * i], w[2 * i + 1]);
+        if constexpr (V == 8) {
+            if (!has(q)) return;
+            Frag<T, 8> f;
+            f.set(w);
+            f.store(p + col(q));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * kPairs; i++)
+                if (in_row() + i * G < d) p[in_row() + i * G] = (T)w[i];
+        }
+    }
+};
+
+// Stages that fit a block's share of shared memory, where `blocks` of them share an SM.
 constexpr int stages(int stage_bytes, int blocks) {
     const int fit = stage_bytes ? 212992 / blocks / stage_bytes : 2;
     return fit > 6 ? 6 : fit;
@@ -192,8 +300,9 @@ constexpr int stages(int stage_bytes, int blocks) {
 // two blocks per SM, or one where that leaves fewer than three stages
 template <typename XT, int V, int P>
 constexpr int kFwdStages = V == 1 ? 2 : stages(kBlock * P * V * (int)sizeof(XT), kBlock * P * V * sizeof(XT) * 6 <= 212992 ? 2 : 1);
+// blocks per SM: what the registers and the stages allow
 template <int P>
-constexpr int kBwdBlocks = P == 1 ? 2 : 1;  // per SM: what the registers allow
+constexpr int kBwdBlocks = P == 1 ? 2 : 1;
 template <typename XT, typename YT, int V, int P>
 constexpr int kBwdStages = V == 1 ? 2 : stages(kBlock * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<P>);
 
@@ -241,37 +350,24 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
     b = __shfl_sync(0xffffffffu, v, 16);
 }
 
-// gamma or beta of this thread's columns: in registers where a thread has one vector, else from cache for every row.
-template <int V, int P>
+// gamma or beta of this thread's columns: in registers where a thread holds 8 elements, else from cache for every row.
+template <int V, int G, int P>
 struct Param {
+    using Mine = Part<V, G, P>;
     static constexpr bool kKept = P * V <= 8;
     const float *p;
-    float kept[kKept ? P : 1][V];
-    __device__ __forceinline__ Param(const float *from, const int (&c)[P], int d, float missing) : p(from) {
+    float missing;
+    f2 kept[kKept ? Mine::kGroups : 1][Mine::kPairs];
+    __device__ __forceinline__ Param(const float *from, const Mine &part, float absent) : p(from), missing(absent) {
         if constexpr (kKept)
 #pragma unroll
-            for (int q = 0; q < P; q++) {
-#pragma unroll
-                for (int i = 0; i < V; i++) kept[q][i] = missing;
-                if (p && c[q] < d) {
-                    Frag<float, V> f;
-                    f.load_cached(p + c[q]);
-                    f.get(kept[q]);
-                }
-            }
+            for (int q = 0; q < Mine::kGroups; q++) part.load(p, q, missing, kept[q]);
     }
-    __device__ __forceinline__ void get(int q, int col, float missing, float (&v)[V]) const {
+    __device__ __forceinline__ void get(const Mine &part, int q, f2 (&v)[Mine::kPairs]) const {
         if constexpr (kKept) {
 #pragma unroll
-            for (int i = 0; i < V; i++) v[i] = kept[q][i];
-        } else if (p) {
-            Frag<float, V> f;
-            f.load_cached(p + col);
-            f.get(v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++) v[i] = missing;
-        }
+            for (int i = 0; i < Mine::kPairs; i++) v[i] = kept[q][i];
+        } else part.load(p, q, missing, v);
     }
 };
 
@@ -279,180 +375,201 @@ template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kBlock, 2)
 norm_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
             YT *__restrict__ y, int64_t ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
+    using Mine = Part<V, G, P>;
+    constexpr int S = kFwdStages<XT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
+    static_assert(S >= 2, "a row is read from one stage while another one fills");
     extern __shared__ __align__(16) char sm[];
     __shared__ float s_sum[2][kBlock / 32];
-    constexpr int S = kFwdStages<XT, V, P>;
-    static_assert(S >= 2, "a row is read from one stage while another one fills");
-    const int group = threadIdx.x / G, in_row = threadIdx.x % G;
-    const int64_t step = (int64_t)gridDim.x * (kBlock / G);
-    int c[P];
-#pragma unroll
-    for (int p = 0; p < P; p++) c[p] = (p * G + in_row) * V;
-    Ahead<XT, V, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), c, d);
-    const float n = (float)d;
+    const int group = threadIdx.x / G;
+    const int step = gridDim.x * (kBlock / G);
+    const Mine part = {d};
+    Ahead<XT, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d);
+    const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, P> scale(gamma, c, d, 1.f), shift(beta, c, d, 0.f);
-    int64_t t = (int64_t)blockIdx.x * (kBlock / G) + group, next = t;
+    const Param<V, G, P> scale(gamma, part, 1.f), shift(beta, part, 0.f);
+    int t = blockIdx.x * (kBlock / G) + group;  // rows of the grid's stride: T + step stays below 2^31, see the launch
+    int next = t;
+    const XT *from = x + (int64_t)t * ldx;
+    YT *to = y + (int64_t)t * ldy;
+    const int64_t from_step = step * ldx, to_step = step * ldy;
 #pragma unroll
-    for (int i = 0; i < S - 1; i++, next += step) {
-        if (next < T) ahead.fetch(i, x + next * ldx, c, d);
+    for (int i = 0; i < S - 1; i++, next += step, from += from_step) {
+        if (next < T) ahead.fetch(i, from, d);
         copies_commit();
     }
     float *s_mean = s_sum[0] + group * (G / 32), *s_var = s_sum[1] + group * (G / 32);
-    for (int stage = 0; t < T; t += step) {
-        float v[P][V], sum = 0.f;
+    for (int stage = 0; t < T; t += step, to += to_step) {
+        f2 v[Q][N], pair = 0ull;
         copies_wait<S - 2>();
-        ahead.take(stage, v);
-        if (next < T) ahead.fetch(stage == 0 ? S - 1 : stage - 1, x + next * ldx, c, d);
+#pragma unroll
+        for (int q = 0; q < Q; q++) ahead.take(stage, q, v[q]);
+        if (next < T) ahead.fetch(stage == 0 ? S - 1 : stage - 1, from, d);
         copies_commit();
         next += step;
+        from += from_step;
         stage = stage + 1 == S ? 0 : stage + 1;
 #pragma unroll
-        for (int p = 0; p < P; p++)
+        for (int q = 0; q < Q; q++)
 #pragma unroll
-            for (int i = 0; i < V; i++) sum += v[p][i];
-        const float mean = row_sum<G>(sum, s_mean) / n;
-        sum = 0.f;
+            for (int i = 0; i < N; i++) pair = add2(pair, v[q][i]);
+        const float mean = row_sum<G>(both(pair), s_mean) * inv;
+        const f2 minus = pack2(-mean, -mean);
+        pair = 0ull;
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (c[p] < d)
+        for (int q = 0; q < Q; q++) {
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    v[p][i] -= mean;
-                    sum = fmaf(v[p][i], v[p][i], sum);
-                }
-        const float rstd = 1.f / sqrtf(row_sum<G>(sum, s_var) / n + eps);
-        if (in_row == 0) {
+            for (int i = 0; i < N; i++) v[q][i] = add2(v[q][i], minus);
+            part.mask(q, v[q]);
+#pragma unroll
+            for (int i = 0; i < N; i++) pair = fma2(v[q][i], v[q][i], pair);
+        }
+        const float rstd = rsqrtf(fmaf(row_sum<G>(both(pair), s_var), inv, eps));
+        if (part.in_row() == 0) {
             if (mean_out) mean_out[t] = mean;
             if (rstd_out) rstd_out[t] = rstd;
         }
+        const f2 r = pack2(rstd, rstd);
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (c[p] < d) {
-                float w[V], b[V];
-                Frag<YT, V> out;
-                scale.get(p, c[p], 1.f, w);
-                shift.get(p, c[p], 0.f, b);
+        for (int q = 0; q < Q; q++) {
+            f2 w[N], b[N];
+            scale.get(part, q, w);
+            shift.get(part, q, b);
 #pragma unroll
-                for (int i = 0; i < V; i++) w[i] = fmaf(v[p][i] * rstd, w[i], b[i]);
-                out.set(w);
-                out.store(y + t * ldy + c[p]);
-            }
+            for (int i = 0; i < N; i++) w[i] = fma2(mul2(v[q][i], r), w[i], b[i]);
+            part.store(to, q, w);
+        }
     }
 }
 
+// The column sums of dy * h and dy stay in registers over all of a block's rows; each block leaves them in `partial`.  With
+// several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
 template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kBlock, kBwdBlocks<P>)
 norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gamma,
                 const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, int64_t lddx,
                 float *__restrict__ partial, int T, int d) {
+    using Mine = Part<V, G, P>;
+    constexpr int S = kBwdStages<XT, YT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
+    constexpr bool kAgain = Q > 1;
+    static_assert(S >= 2, "a row is read from one stage while another one fills");
     extern __shared__ __align__(16) char sm[];
     __shared__ float s_sum[2][2 * kBlock / 32];
-    constexpr int S = kBwdStages<XT, YT, V, P>;
-    static_assert(S >= 2, "a row is read from one stage while another one fills");
-    const int group = threadIdx.x / G, in_row = threadIdx.x % G;
-    const int64_t step = (int64_t)gridDim.x * (kBlock / G);
-    int c[P];
-    float dg[P][V], db[P][V];
+    const int group = threadIdx.x / G;
+    const int step = gridDim.x * (kBlock / G);
+    const Mine part = {d};
+    f2 dg[Q][N], db[Q][N];
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-        c[p] = (p * G + in_row) * V;
+    for (int q = 0; q < Q; q++)
 #pragma unroll
-        for (int i = 0; i < V; i++) dg[p][i] = db[p][i] = 0.f;
-    }
+        for (int i = 0; i < N; i++) dg[q][i] = db[q][i] = 0ull;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm);
-    Ahead<XT, V, P, S> ahead_x(ring, c, d);
-    Ahead<YT, V, P, S> ahead_y(ring + S * Ahead<XT, V, P, S>::kStage, c, d);
-    const float n = (float)d;
+    Ahead<XT, V, G, P, S> ahead_x(ring, d);
+    Ahead<YT, V, G, P, S> ahead_y(ring + S * Ahead<XT, V, G, P, S>::kStage, d);
+    const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, P> scale(gamma, c, d, 1.f);
-    int64_t t = (int64_t)blockIdx.x * (kBlock / G) + group, next = t;
-#pragma unroll
-    for (int i = 0; i < S - 1; i++, next += step) {
+    const Param<V, G, P> scale(gamma, part, 1.f);
+    int t = blockIdx.x * (kBlock / G) + group, next = t;
+    const XT *from_x = x + (int64_t)t * ldx;
+    const YT *from_y = dy + (int64_t)t * lddy;
+    XT *to = dx + (int64_t)t * lddx;
+    const int64_t x_step = step * ldx, y_step = step * lddy, to_step = step * lddx;
+    auto fetch = [&](int stage) {
         if (next < T) {
-            ahead_x.fetch(i, x + next * ldx, c, d);
-            ahead_y.fetch(i, dy + next * lddy, c, d);
+            ahead_x.fetch(stage, from_x, d);
+            ahead_y.fetch(stage, from_y, d);
         }
         copies_commit();
-    }
+        next += step;
+        from_x += x_step;
+        from_y += y_step;
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) fetch(i);
     float m = 0.f, r = 0.f;
     if (t < T) {
         m = mean[t];
         r = rstd[t];
     }
-    for (int stage = 0, odd = 0; t < T; t += step, odd ^= 1) {
-        float h[P][V], g[P][V], mg = 0.f, mh = 0.f;
-        copies_wait<S - 2>();
-        ahead_x.take(stage, h);
-        ahead_y.take(stage, g);
-        if (next < T) {
-            const int to = stage == 0 ? S - 1 : stage - 1;
-            ahead_x.fetch(to, x + next * ldx, c, d);
-            ahead_y.fetch(to, dy + next * lddy, c, d);
-        }
-        copies_commit();
-        next += step;
-        stage = stage + 1 == S ? 0 : stage + 1;
-        const float m0 = m, r0 = r;
+    for (int stage = 0, odd = 0; t < T; t += step, to += to_step, odd ^= 1) {
+        f2 h[Q][N], g[Q][N], sum_g = 0ull, sum_gh = 0ull;
+        const f2 minus = pack2(-m, -m), rr = pack2(r, r);
+        const int refill = stage == 0 ? S - 1 : stage - 1;
         if (t + step < T) {
             m = mean[t + step];
             r = rstd[t + step];
         }
+        copies_wait<S - 2>();
+        if constexpr (!kAgain) {
+            ahead_x.take(stage, 0, h[0]);
+            ahead_y.take(stage, 0, g[0]);
+        }
+        fetch(refill);
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (c[p] < d) {
-                float w[V];
-                scale.get(p, c[p], 1.f, w);
+        for (int q = 0; q < Q; q++) {
+            if constexpr (kAgain) {
+                ahead_x.take(stage, q, h[q]);
+                ahead_y.take(stage, q, g[q]);
+            }
+            f2 w[N];
+            scale.get(part, q, w);
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    h[p][i] = (h[p][i] - m0) * r0;
-                    dg[p][i] = fmaf(g[p][i], h[p][i], dg[p][i]);
-                    db[p][i] += g[p][i];
-                    g[p][i] *= w[i];
-                    mg += g[p][i];
-                    mh = fmaf(g[p][i], h[p][i], mh);
+            for (int i = 0; i < N; i++) {
+                h[q][i] = mul2(add2(h[q][i], minus), rr);
+                dg[q][i] = fma2(g[q][i], h[q][i], dg[q][i]);
+                db[q][i] = add2(db[q][i], g[q][i]);
+                g[q][i] = mul2(g[q][i], w[i]);
+                sum_g = add2(sum_g, g[q][i]);
+                sum_gh = fma2(g[q][i], h[q][i], sum_gh);
+            }
+        }
+        float mg = both(sum_g), mh = both(sum_gh);
+        row_sums<G>(mg, mh, s_sum[odd] + group * (2 * G / 32));
+        const f2 less = pack2(-mg * inv, -mg * inv), slope = pack2(-mh * inv, -mh * inv);
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            f2 out[N];
+            if constexpr (kAgain) {
+                f2 w[N];
+                ahead_x.take(stage, q, h[q]);
+                ahead_y.take(stage, q, g[q]);
+                scale.get(part, q, w);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    h[q][i] = mul2(add2(h[q][i], minus), rr);
+                    g[q][i] = mul2(g[q][i], w[i]);
                 }
             }
-        row_sums<G>(mg, mh, s_sum[odd] + group * (2 * G / 32));
-        mg /= n;
-        mh /= n;
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (c[p] < d) {
-                Frag<XT, V> out;
-                float v[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) v[i] = r0 * fmaf(-h[p][i], mh, g[p][i] - mg);
-                out.set(v);
-                out.store(dx + t * lddx + c[p]);
-            }
+            for (int i = 0; i < N; i++) out[i] = mul2(fma2(h[q][i], slope, add2(g[q][i], less)), rr);
+            part.store(to, q, out);
+        }
+        stage = stage + 1 == S ? 0 : stage + 1;
     }
     if (!partial) return;
     // column sums of the block: the rows' groups joined through shared memory, in order
-    float *to = partial + (int64_t)blockIdx.x * 2 * d;
+    float *sums = partial + (int64_t)blockIdx.x * 2 * d;
     if constexpr (G == kBlock) {
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (c[p] < d) {
-                Frag<float, V> f;
-                f.set(dg[p]);
-                f.store(to + c[p]);
-                f.set(db[p]);
-                f.store(to + d + c[p]);
-            }
+        for (int q = 0; q < Q; q++) {
+            part.store(sums, q, dg[q]);
+            part.store(sums + d, q, db[q]);
+        }
     } else {
         constexpr int W = G * P * V;  // columns a group covers
         float *s = reinterpret_cast<float *>(sm);
+        const Mine whole = {W};
         copies_wait<0>();
         __syncthreads();
 #pragma unroll
-        for (int p = 0; p < P; p++)
+        for (int q = 0; q < Q; q++)
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                s[(group * 2) * W + c[p] + i] = dg[p][i];
-                s[(group * 2 + 1) * W + c[p] + i] = db[p][i];
+            for (int i = 0; i < N; i++) {
+                const int c = V == 8 ? whole.col(q) + 2 * i : whole.in_row() + 2 * i * G, next_c = V == 8 ? 1 : G;
+                float *a = s + group * 2 * W + c, *b = a + W;
+                unpack2(dg[q][i], a[0], a[next_c]);
+                unpack2(db[q][i], b[0], b[next_c]);
             }
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * W; i += kBlock) {
@@ -461,7 +578,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ 
             float sum = 0.f;
 #pragma unroll
             for (int q = 0; q < kBlock / G; q++) sum += s[(q * 2 + which) * W + col];
-            to[which * d + col] = sum;
+            sums[which * d + col] = sum;
         }
     }
 }
@@ -541,6 +658,7 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
                     void *cuda_stream) {
     const char *fn = "omoe_layer_norm";
     if (T < 0) return ops_fail(OMOE_ERR_INVALID, fn, "T must not be negative");
+    if (T > kRowsMax) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "T is beyond the limit");
     if (!(eps >= 0.f)) return ops_fail(OMOE_ERR_INVALID, fn, "eps must not be negative");
     const Rows x = {x_dev, ldx, x_dtype, T, d}, y = {y_dev, ldy, y_dtype, T, d};
     if (const char *bad = rows_wrong(x)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
@@ -556,10 +674,10 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
         using XT = std::remove_pointer_t<decltype(xt)>;
         using YT = std::remove_pointer_t<decltype(yt)>;
         cudaError_t e = cudaSuccess;
-        if (by_width(rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 16) && !misaligned(beta_dev, 16), d,
+        if (by_width(rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 32) && !misaligned(beta_dev, 32), d,
                      [&](auto v, auto g, auto p) {
                          constexpr int V = decltype(v)::value, G = decltype(g)::value, P = decltype(p)::value;
-                         constexpr size_t smem = kFwdStages<XT, V, P> * Ahead<XT, V, P, 2>::kStage;
+                         constexpr size_t smem = kFwdStages<XT, V, P> * Ahead<XT, V, G, P, 2>::kStage;
                          static PerDeviceOnce once;
                          e = allow_smem(norm_kernel<XT, YT, V, G, P>, smem, once);
                          if (e != cudaSuccess) return;
@@ -585,6 +703,7 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
                              int64_t workspace_bytes, void *cuda_stream) {
     const char *fn = "omoe_layer_norm_backward";
     if (T < 0) return ops_fail(OMOE_ERR_INVALID, fn, "T must not be negative");
+    if (T > kRowsMax) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "T is beyond the limit");
     const Rows dx = {dx_dev, lddx, x_dtype, T, d}, dy = {dy_dev, lddy, dy_dtype, T, d}, x = {x_dev, ldx, x_dtype, T, d};
     for (const Rows *r : {&dx, &dy, &x})
         if (const char *bad = rows_wrong(*r)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
@@ -593,7 +712,7 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
     if (misaligned(gamma_dev, 4) || misaligned(mean_dev, 4) || misaligned(rstd_dev, 4) || misaligned(dgamma_dev, 4) ||
         misaligned(dbeta_dev, 4))
         return ops_fail(OMOE_ERR_INVALID, fn, "fp32 buffers must be 4-byte aligned");
-    if (workspace_bytes < omoe_layer_norm_backward_workspace(T, d) || !workspace_dev || misaligned(workspace_dev, 16))
+    if (workspace_bytes < omoe_layer_norm_backward_workspace(T, d) || !workspace_dev || misaligned(workspace_dev, 32))
         return ops_fail(OMOE_ERR_INVALID, fn, "the workspace is missing, misaligned or too small");
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     const int sms = ops_sm_count();
@@ -608,12 +727,12 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
         const XT *in = static_cast<const XT *>(x_dev);
         cudaError_t e = cudaSuccess;
         int sums = 0;  // column sums in the workspace
-        if (T > 0 && by_width(rows_vector(x) && rows_vector(dy) && rows_vector(dx) && !misaligned(gamma_dev, 16), d,
+        if (T > 0 && by_width(rows_vector(x) && rows_vector(dy) && rows_vector(dx) && !misaligned(gamma_dev, 32), d,
                               [&](auto v, auto gg, auto p) {
                                   constexpr int V = decltype(v)::value, G = decltype(gg)::value, P = decltype(p)::value;
                                   constexpr int S = kBwdStages<XT, YT, V, P>;
                                   if constexpr (S >= 2) {
-                                      constexpr size_t ring = S * (Ahead<XT, V, P, S>::kStage + Ahead<YT, V, P, S>::kStage);
+                                      constexpr size_t ring = S * (Ahead<XT, V, G, P, S>::kStage + Ahead<YT, V, G, P, S>::kStage);
                                       constexpr size_t join = G < kBlock ? 2 * kBlock * P * V * sizeof(float) : 0;
                                       constexpr size_t smem = ring > join ? ring : join;
                                       static PerDeviceOnce once;

@@ -29,9 +29,9 @@ struct Rows {
 const char *rows_wrong(const Rows &r);
 // True where an element of `a` is also one of `b`.  Two column windows of the same matrix do not overlap.
 bool rows_overlap(const Rows &a, const Rows &b);
-// True when every group of 8 elements of a row is 16-byte aligned, for all of the matrices.
+// True when every group of 8 elements of a row is aligned to its size (16 bytes of bf16, 32 of fp32).
 inline bool rows_vector(const Rows &r) {
-    return r.d % 8 == 0 && (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && (r.rows <= 1 || (r.ld * r.elem()) % 16 == 0);
+    return r.d % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % (8 * r.elem()) == 0 && (r.rows <= 1 || r.ld % 8 == 0);
 }
 inline bool misaligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
@@ -57,26 +57,31 @@ struct Frag<__nv_bfloat16, 8> {
 };
 template <>
 struct Frag<float, 8> {
-    float4 a, b;
+    // one 32-byte access: two of 16 bytes would each touch half of every 32-byte sector of the warp's lines
+    float r[8];
     __device__ __forceinline__ void load(const float *p) {
-        a = __ldcs(reinterpret_cast<const float4 *>(p));
-        b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+        asm volatile("ld.global.cs.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "l"(p) : "memory");
     }
     __device__ __forceinline__ void load_cached(const float *p) {
-        a = __ldg(reinterpret_cast<const float4 *>(p));
-        b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "l"(p));
     }
     __device__ __forceinline__ void store(float *p) const {
-        *reinterpret_cast<float4 *>(p) = a;
-        *(reinterpret_cast<float4 *>(p) + 1) = b;
+        asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]),
+                     "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "l"(p) : "memory");
     }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = 0.f;
+    }
     __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = r[i];
     }
     __device__ __forceinline__ void set(const float (&v)[8]) {
-        a = make_float4(v[0], v[1], v[2], v[3]);
-        b = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = v[i];
     }
 };
 template <>
