@@ -161,49 +161,54 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
     return r;
 }
 
-// The rows ahead.  V = 8: S stages of shared memory; a stage holds, for every vector of a thread, a plane of 16 bytes per
-// thread (two for fp32).  fp32 is copied by the lanes of a warp in the order of the addresses, not of the owners: 16 of the
-// owner's 32 bytes at a time would move every sector twice.
+// The rows ahead.  V = 8: S stages of shared memory.  In a stage every warp has, for each vector of its threads, the 256 columns
+// they hold as they lie in the row, in pieces of 16 bytes; the lanes copy neighbouring pieces.  A thread's 8 columns are one
+// piece of bf16 and two of fp32; there pieces 8 .. 15 of every 16 are swapped in pairs, so that eight lanes reading their first
+// pieces meet all banks.
 // V = 1 (rows that are not aligned): one row ahead, in registers.
 template <typename T, int V, int G, int P, int S>
 struct Ahead {
-    static constexpr int kPlanes = sizeof(T) / 2;
-    static constexpr int kStage = kBlock * 16 * kPlanes * P;
-    uint32_t own, put;  // this thread's slot, and where it puts what it copies
-    int col;            // the first column it copies
+    static constexpr int kPieces = sizeof(T) / 2;  // of a thread's vector
+    static constexpr int kVector = kBlock * 16 * kPieces, kStage = kVector * P;
+    uint32_t first, second, put;  // this thread's pieces, and where it puts what it copies
+    int col;                      // the first column it copies
     // vectors behind the row's end are zeros in every stage from the start
     __device__ __forceinline__ Ahead(uint32_t ring, int d) {
         const int lane = threadIdx.x & 31, in_row = threadIdx.x % G;
-        own = ring + threadIdx.x * 16;
-        put = kPlanes == 1 ? own : ring + (lane & 1) * (kBlock * 16) + (threadIdx.x - (lane + 1) / 2) * 16;
-        col = kPlanes == 1 ? in_row * 8 : (in_row - lane) * 8 + lane * 4;
+        const uint32_t warp = ring + (threadIdx.x - lane) * 16 * kPieces;
+        const int swap = kPieces == 2 ? lane >> 2 & 1 : 0;
+        first = warp + (lane * kPieces ^ swap) * 16;
+        second = warp + ((lane * kPieces + 1) ^ swap) * 16;
+        put = warp + (kPieces == 2 ? lane ^ (lane >> 3 & 1) : lane) * 16;
+        col = (in_row - lane) * 8 + lane * (8 / kPieces);
 #pragma unroll
         for (int p = 0; p < P; p++)
             if ((p * G + in_row) * 8 >= d)
-                for (int i = 0; i < S; i++)
-#pragma unroll
-                    for (int q = 0; q < kPlanes; q++)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(own + i * kStage + (p * kPlanes + q) * (kBlock * 16)), "r"(0) : "memory");
+                for (int i = 0; i < S; i++) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(first + i * kStage + p * kVector), "r"(0) : "memory");
+                    if constexpr (kPieces == 2)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(second + i * kStage + p * kVector), "r"(0) : "memory");
+                }
         __syncwarp();
     }
     __device__ __forceinline__ void fetch(int stage, const T *row, int d) const {
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int q = 0; q < kPlanes; q++) {
+            for (int q = 0; q < kPieces; q++) {
                 const int c = col + p * G * 8 + q * 128;
-                if (c < d) copy16(put + stage * kStage + p * kPlanes * (kBlock * 16) + q * 256, row + c);
+                if (c < d) copy16(put + stage * kStage + p * kVector + q * 512, row + c);
             }
     }
     // pairs 4p .. 4p + 3 of this thread
     __device__ __forceinline__ void take(int stage, int p, f2 (&v)[4]) const {
-        const uint4 a = shared16(own + stage * kStage + p * kPlanes * (kBlock * 16));
-        if constexpr (kPlanes == 1) {
+        const uint4 a = shared16(first + stage * kStage + p * kVector);
+        if constexpr (kPieces == 1) {
             const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
             for (int i = 0; i < 4; i++) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
         } else {
-            const uint4 b = shared16(own + stage * kStage + (p * kPlanes + 1) * (kBlock * 16));
+            const uint4 b = shared16(second + stage * kStage + p * kVector);
             v[0] = pack2(__uint_as_float(a.x), __uint_as_float(a.y));
             v[1] = pack2(__uint_as_float(a.z), __uint_as_float(a.w));
             v[2] = pack2(__uint_as_float(b.x), __uint_as_float(b.y));
@@ -373,8 +378,8 @@ struct Param {
 
 template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kBlock, 2)
-norm_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
-            YT *__restrict__ y, int64_t ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
+norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
+            YT *__restrict__ y, int ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
     using Mine = Part<V, G, P>;
     constexpr int S = kFwdStages<XT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
     static_assert(S >= 2, "a row is read from one stage while another one fills");
@@ -390,24 +395,20 @@ norm_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gam
     const Param<V, G, P> scale(gamma, part, 1.f), shift(beta, part, 0.f);
     int t = blockIdx.x * (kBlock / G) + group;  // rows of the grid's stride: T + step stays below 2^31, see the launch
     int next = t;
-    const XT *from = x + (int64_t)t * ldx;
-    YT *to = y + (int64_t)t * ldy;
-    const int64_t from_step = step * ldx, to_step = step * ldy;
-#pragma unroll
-    for (int i = 0; i < S - 1; i++, next += step, from += from_step) {
-        if (next < T) ahead.fetch(i, from, d);
+    auto fetch = [&](int stage) {
+        if (next < T) ahead.fetch(stage, x + (int64_t)next * ldx, d);
         copies_commit();
-    }
+        next += step;
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) fetch(i);
     float *s_mean = s_sum[0] + group * (G / 32), *s_var = s_sum[1] + group * (G / 32);
-    for (int stage = 0; t < T; t += step, to += to_step) {
+    for (int stage = 0; t < T; t += step) {
         f2 v[Q][N], pair = 0ull;
         copies_wait<S - 2>();
 #pragma unroll
         for (int q = 0; q < Q; q++) ahead.take(stage, q, v[q]);
-        if (next < T) ahead.fetch(stage == 0 ? S - 1 : stage - 1, from, d);
-        copies_commit();
-        next += step;
-        from += from_step;
+        fetch(stage == 0 ? S - 1 : stage - 1);
         stage = stage + 1 == S ? 0 : stage + 1;
 #pragma unroll
         for (int q = 0; q < Q; q++)
@@ -437,7 +438,7 @@ norm_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gam
             shift.get(part, q, b);
 #pragma unroll
             for (int i = 0; i < N; i++) w[i] = fma2(mul2(v[q][i], r), w[i], b[i]);
-            part.store(to, q, w);
+            part.store(y + (int64_t)t * ldy, q, w);
         }
     }
 }
@@ -446,8 +447,8 @@ norm_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gam
 // several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
 template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kBlock, kBwdBlocks<P>)
-norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gamma,
-                const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, int64_t lddx,
+norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, int ldx, const float *__restrict__ gamma,
+                const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, int lddx,
                 float *__restrict__ partial, int T, int d) {
     using Mine = Part<V, G, P>;
     constexpr int S = kBwdStages<XT, YT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
@@ -471,19 +472,13 @@ norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ 
     pdl_wait();
     const Param<V, G, P> scale(gamma, part, 1.f);
     int t = blockIdx.x * (kBlock / G) + group, next = t;
-    const XT *from_x = x + (int64_t)t * ldx;
-    const YT *from_y = dy + (int64_t)t * lddy;
-    XT *to = dx + (int64_t)t * lddx;
-    const int64_t x_step = step * ldx, y_step = step * lddy, to_step = step * lddx;
     auto fetch = [&](int stage) {
         if (next < T) {
-            ahead_x.fetch(stage, from_x, d);
-            ahead_y.fetch(stage, from_y, d);
+            ahead_x.fetch(stage, x + (int64_t)next * ldx, d);
+            ahead_y.fetch(stage, dy + (int64_t)next * lddy, d);
         }
         copies_commit();
         next += step;
-        from_x += x_step;
-        from_y += y_step;
     };
 #pragma unroll
     for (int i = 0; i < S - 1; i++) fetch(i);
@@ -492,7 +487,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ 
         m = mean[t];
         r = rstd[t];
     }
-    for (int stage = 0, odd = 0; t < T; t += step, to += to_step, odd ^= 1) {
+    for (int stage = 0, odd = 0; t < T; t += step, odd ^= 1) {
         f2 h[Q][N], g[Q][N], sum_g = 0ull, sum_gh = 0ull;
         const f2 minus = pack2(-m, -m), rr = pack2(r, r);
         const int refill = stage == 0 ? S - 1 : stage - 1;
@@ -543,7 +538,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ 
             }
 #pragma unroll
             for (int i = 0; i < N; i++) out[i] = mul2(fma2(h[q][i], slope, add2(g[q][i], less)), rr);
-            part.store(to, q, out);
+            part.store(dx + (int64_t)t * lddx, q, out);
         }
         stage = stage + 1 == S ? 0 : stage + 1;
     }
@@ -683,7 +678,7 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
                          if (e != cudaSuccess) return;
                          const int blocks = ceil_div(T, kBlock / G), most = 2 * sms;
                          e = launch_ex(norm_kernel<XT, YT, V, G, P>, dim3(blocks < most ? blocks : most), dim3(kBlock), smem, s, ops_pdl(),
-                                       static_cast<const XT *>(x_dev), ldx, gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev), ldy,
+                                       static_cast<const XT *>(x_dev), (int)ldx, gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev), (int)ldy,
                                        mean_dev, rstd_dev, T, d);
                      }))
             return e;
@@ -742,8 +737,8 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
                                       int most = kBwdBlocks<P> * sms;
                                       most = most < kBwdBlocksMax ? most : kBwdBlocksMax;
                                       sums = blocks < most ? blocks : most;
-                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(kBlock), smem, s, ops_pdl(), g, lddy, in,
-                                                    ldx, gamma_dev, mean_dev, rstd_dev, static_cast<XT *>(dx_dev), lddx,
+                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(kBlock), smem, s, ops_pdl(), g, (int)lddy, in,
+                                                    (int)ldx, gamma_dev, mean_dev, rstd_dev, static_cast<XT *>(dx_dev), (int)lddx,
                                                     params ? partial : nullptr, T, d);
                                   }
                               }) && (e != cudaSuccess || sums > 0)) {
