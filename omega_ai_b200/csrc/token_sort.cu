@@ -17,23 +17,32 @@ constexpr int64_t kRowsMax = 0x7fff0000;  // row numbers, and a block's worth be
 constexpr int kPlanWarps = 32;
 constexpr int kPlanBatch = 8;    // picks a lane loads together
 constexpr int kPlanCtasMax = 8;  // the portable cluster size
+constexpr size_t kPlanSmem = 220 * 1024;
+static_assert(sizeof(int32_t) * (OMOE_SORT_MAX_EXPERTS * (5 + kPlanWarps) + 1) <= kPlanSmem, "the tables of the most experts fit");
 
 // One cluster does the whole plan.  Every warp owns a contiguous run of picks and counts its picks of every expert in
 // shared memory, numbering them as it goes: lanes with the same expert are found by ballots over the bits of its number (a warp-wide
 // match takes longer the more experts meet in a warp).  After sums over the warps and, through distributed shared memory,
 // over the CTAs every warp knows where its first pick of each expert goes.  A run of up to 256 picks stays in
-// registers, a longer one keeps its numbers in pos meanwhile.  Bound by latency: the walk and the barriers.
+// registers, a longer one keeps its numbers in pos meanwhile.
+// perm is a scatter: written pick by pick every store touches up to 32 lines, and eight SMs have to make them all (5 of 13 us for 49152
+// picks on 64 experts).  So the CTA's picks are put in order in shared memory first, `list` of them at most, and leave
+// as one run per expert.  Bound by latency: the walk, the barriers, the copies.
 __global__ void __launch_bounds__(kPlanWarps * 32)
-sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int rows_cap, int warp_run,
+sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int rows_cap, int warp_run, int list,
                  int32_t *__restrict__ pos, int32_t *__restrict__ perm, int32_t *__restrict__ counts,
                  int32_t *__restrict__ offsets) {
     extern __shared__ int32_t sm[];
     cg::cluster_group cluster = cg::this_cluster();
     const int nw = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int32_t *s_total = sm;             // [E] this CTA's picks of every expert, read by the others
-    int32_t *s_count = s_total + E;    // [E] all picks
-    int32_t *s_start = s_count + E;    // [E+1] first row of every expert
-    int32_t *s_hist = s_start + E + 1; // [warps][E]
+    int32_t *s_total = sm;              // [E] this CTA's picks of every expert, read by the others
+    int32_t *s_count = s_total + E;     // [E] all picks
+    int32_t *s_first = s_count + E;     // [E+1] first row of every expert
+    int32_t *s_start = s_first + E + 1; // [E] first row of this CTA's picks of the expert
+    int32_t *s_local = s_start + E;     // [E] where they start in the CTA's list
+    int32_t *s_hist = s_local + E;      // [warps][E]
+    int32_t *s_list = s_hist + nw * E;  // [list] pick numbers by expert
+    uint16_t *s_expert = reinterpret_cast<uint16_t *>(s_list + list);  // [list]
     int32_t *hist = s_hist + warp * E;
     const int ctas = cluster.num_blocks(), cta = cluster.block_rank();
 
@@ -73,7 +82,7 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int run = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int w = 0; w < nw; w++) {
             const int c = s_hist[w * E + e];
             s_hist[w * E + e] = run;
@@ -85,7 +94,9 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     else __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int before = 0, all = 0;
-        for (int c = 0; c < ctas; c++) {
+#pragma unroll
+        for (int c = 0; c < kPlanCtasMax; c++) {
+            if (c >= ctas) break;
             const int v = c == cta ? s_total[e] : cluster.map_shared_rank(s_total, c)[e];
             if (c < cta) before += v;
             all += v;
@@ -95,61 +106,86 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     }
     __syncthreads();
     if (warp == 0) {
-        int row = 0;
+        int row = 0, local = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
             const int e = e0 + lane;
-            const int c = e < E ? s_count[e] : 0, p = (c + align - 1) / align * align;
-            int inc = p;
+            const int c = e < E ? s_total[e] : 0, p = e < E ? (s_count[e] + align - 1) / align * align : 0;
+            int rows = p, mine = c;  // inclusive sums over the lanes
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
+                const int r = __shfl_up_sync(0xffffffffu, rows, o), m = __shfl_up_sync(0xffffffffu, mine, o);
+                if (lane >= o) { rows += r; mine += m; }
             }
             if (e < E) {
-                const int first = row + inc - p;
-                s_start[e] += first;
-                if (cta == 0) {
-                    counts[e] = c;
-                    offsets[e] = first;
-                }
-                // padding rows have no pick; the CTAs share the experts
-                if (e % ctas == cta)
-                    for (int r = first + c; r < first + p && r < rows_cap; r++) perm[r] = -1;
+                s_first[e] = row + rows - p;
+                s_start[e] += row + rows - p;
+                s_local[e] = local + mine - c;
             }
-            row += __shfl_sync(0xffffffffu, inc, 31);
+            row += __shfl_sync(0xffffffffu, rows, 31);
+            local += __shfl_sync(0xffffffffu, mine, 31);
         }
-        if (lane == 0) {
-            s_start[E] = row;
-            if (cta == 0) offsets[E] = row;
-        }
+        if (lane == 0) s_first[E] = row;
     }
     __syncthreads();
-    for (int64_t r = (int64_t)s_start[E] + cta * blockDim.x + threadIdx.x; r < rows_cap; r += ctas * blockDim.x) perm[r] = -1;
     for (int i0 = lo; i0 < hi; i0 += kPlanBatch * 32) {
         if (warp_run > kPlanBatch * 32) {
 #pragma unroll
             for (int u = 0; u < kPlanBatch; u++) {
                 const int i = i0 + u * 32 + lane;
-                key[u] = i < hi ? idx[i] : -1;
+                const int e = i < hi ? idx[i] : -1;
+                key[u] = e >= 0 && e < E ? e : E;
                 rank[u] = i < hi ? pos[i] : 0;
             }
         }
 #pragma unroll
         for (int u = 0; u < kPlanBatch; u++) {
-            const int i = i0 + u * 32 + lane;
+            const int i = i0 + u * 32 + lane, e = key[u];
             if (i >= hi) continue;
             int row = -1;
-            if (key[u] >= 0 && key[u] < E) row = s_start[key[u]] + hist[key[u]] + rank[u];
+            if (e < E) {
+                const int q = hist[e] + rank[u];  // among the CTA's picks of the expert
+                row = s_start[e] + q;
+                if (list) {
+                    s_list[s_local[e] + q] = i;
+                    s_expert[s_local[e] + q] = (uint16_t)e;
+                } else if (row < rows_cap) perm[row] = i;
+            }
             pos[i] = row;
-            if (row >= 0 && row < rows_cap) perm[row] = i;
+        }
+    }
+    // what is the same for all CTAs is shared out: counts and offsets, and perm where there is no pick
+    for (int e = cta * blockDim.x + threadIdx.x; e < E; e += ctas * blockDim.x) {
+        counts[e] = s_count[e];
+        offsets[e] = s_first[e];
+    }
+    if (cta == 0 && threadIdx.x == 0) offsets[E] = s_first[E];
+    for (int e = align > 1 ? cta * nw + warp : E; e < E; e += ctas * nw)
+        for (int r = s_first[e] + s_count[e] + lane; r < s_first[e + 1] && r < rows_cap; r += 32) perm[r] = -1;
+    for (int64_t r = (int64_t)s_first[E] + cta * blockDim.x + threadIdx.x; r < rows_cap; r += ctas * blockDim.x) perm[r] = -1;
+    if (list) {
+        __syncthreads();
+        const int mine = s_local[E - 1] + s_total[E - 1];
+        for (int q = threadIdx.x; q < mine; q += blockDim.x) {
+            const int e = s_expert[q], row = s_start[e] + q - s_local[e];
+            if (row < rows_cap) perm[row] = s_list[q];
         }
     }
     if (ctas > 1) cluster.sync();  // the others may still read this CTA's totals
 }
 
-// A warp takes one chunk of a token's columns: U vectors per lane.
-template <int V>
-constexpr int kChunk = 32 * V * (V == 8 ? 4 : 8);
+// A warp takes one chunk of a token's columns: U vectors per lane.  Narrow rows get fewer (a warp that has nothing to do for most of
+// its vectors still issues for them: 20 us against 11 for 16384 tokens of 128 columns and 8 picks).
+template <int V, int U>
+constexpr int kChunk = 32 * V * U;
+// Calls f(V, U) (integral constants) for rows of width d.
+template <typename F>
+int by_chunk(bool vec, int d, F f) {
+    using std::integral_constant;
+    if (!vec) return f(integral_constant<int, 1>(), integral_constant<int, 8>());
+    if (d <= 256) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    if (d <= 512) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
+    return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+}
 
 // The rows of a token's picks, a pick per lane; picks without a row, or with one that no plan makes, are negative.
 __device__ __forceinline__ int pick_row(const int32_t *pos, int64_t t, int k, int lane, int rows_cap) {
@@ -182,21 +218,20 @@ __device__ __forceinline__ void zero_padding(T *rows, int64_t ld, const int32_t 
 }
 
 // xs[pos] = x: a warp reads a chunk of a token's row once and stores it for every pick.  HBM bound.
-template <typename XT, typename OT, int V>
+template <typename XT, typename OT, int V, int U>
 __global__ void __launch_bounds__(256)
 sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int64_t ldxs, const int32_t *__restrict__ pos,
                  const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int T, int k, int pads, int slices, int d,
                  int n_chunks, int rows_cap) {
-    constexpr int U = kChunk<V> / (32 * V);
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t t = item / n_chunks;
-    const int c0 = (int)(item % n_chunks) * kChunk<V> + lane * V;
+    const int c0 = (int)(item % n_chunks) * kChunk<V, U> + lane * V;
     pdl_trigger();
     pdl_wait();
     if (t >= T) {
         if (t - T < pads)
-            zero_padding<OT, V>(xs, ldxs, counts, offsets, (int)(t - T), slices, c0, min(d, c0 - lane * V + kChunk<V>), 32 * V, rows_cap);
+            zero_padding<OT, V>(xs, ldxs, counts, offsets, (int)(t - T), slices, c0, min(d, c0 - lane * V + kChunk<V, U>), 32 * V, rows_cap);
         return;
     }
     const int r = pick_row(pos, t, k, lane, rows_cap);
@@ -219,15 +254,14 @@ sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int
 
 // y[t] = sum over the picks of w * ys[pos] (W) or of ys[pos]: a warp per chunk of a token's columns, two picks' loads in
 // flight.  fp32 sums in pick order.  HBM bound.
-template <typename XT, typename OT, int V, bool W>
+template <typename XT, typename OT, int V, int U, bool W>
 __global__ void __launch_bounds__(256)
 unsort_rows_kernel(const XT *__restrict__ ys, int64_t ldys, OT *__restrict__ y, int64_t ldy, const int32_t *__restrict__ pos,
                    const float *__restrict__ w, int T, int k, int d, int n_chunks, int rows_cap) {
-    constexpr int U = kChunk<V> / (32 * V);
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t t = item / n_chunks;
-    const int c0 = (int)(item % n_chunks) * kChunk<V> + lane * V;
+    const int c0 = (int)(item % n_chunks) * kChunk<V, U> + lane * V;
     pdl_trigger();
     pdl_wait();
     if (t >= T) return;
@@ -278,55 +312,60 @@ unsort_rows_kernel(const XT *__restrict__ ys, int64_t ldys, OT *__restrict__ y, 
         }
 }
 
-// dys[pos] = w * dy and dw = <dy, ys[pos]>: a block per token reads dy once; a thread's columns are added up for every
-// pick in registers, then over the warp and the block in a fixed order.  K bounds k.  HBM bound.
+// dys[pos] = w * dy and dw = <dy, ys[pos]>: `threads` threads per token read dy once; a thread's columns are
+// added up for every pick in registers, then over the token's threads in a fixed order.  K bounds k.  HBM bound.
 template <typename DT, typename YT, int V, int K>
 __global__ void __launch_bounds__(512)
 unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict__ ys, int64_t ldys, YT *__restrict__ dys,
                   int64_t lddys, const int32_t *__restrict__ pos, const int32_t *__restrict__ counts,
-                  const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int slices,
-                  int d, int rows_cap) {
+                  const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int pads,
+                  int slices, int d, int rows_cap, int threads) {
+    constexpr int J = K <= 6 || (sizeof(YT) * V <= 16 && K <= 8) ? K : 4;  // picks whose vectors are held at a time
     __shared__ float s_dot[16][K];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, of_token = threadIdx.x % threads;
+    const int64_t t = (int64_t)blockIdx.x * (blockDim.x / threads) + threadIdx.x / threads;
     pdl_trigger();
     pdl_wait();
-    if (t >= T) {
-        zero_padding<YT, V>(dys, lddys, counts, offsets, (int)(t - T), slices, threadIdx.x * V, d, blockDim.x * V, rows_cap);
-        return;
-    }
-    int row[K];
-    float wt[K], dot[K];
+    if (t >= T && t - T < pads) zero_padding<YT, V>(dys, lddys, counts, offsets, (int)(t - T), slices, of_token * V, d, threads * V, rows_cap);
+    float dot[K];
 #pragma unroll
-    for (int j = 0; j < K; j++) {
-        row[j] = j < k ? pos[t * k + j] : -1;
-        if (row[j] >= rows_cap) row[j] = -1;
-        wt[j] = w && j < k ? w[t * k + j] : 1.f;
-        dot[j] = 0.f;
-    }
-    for (int c = threadIdx.x * V; c < d; c += blockDim.x * V) {
-        Frag<DT, V> g;
-        Frag<YT, V> y[K], o;
-        g.load(dy + t * lddy + c);
-        if (dw)
+    for (int j = 0; j < K; j++) dot[j] = 0.f;
+    if (t < T) {
+        int row[K];
+        float wt[K];
 #pragma unroll
-            for (int j = 0; j < K; j++)
-                if (row[j] >= 0) y[j].load(ys + (int64_t)row[j] * ldys + c);
-        float gv[V], v[V];
-        g.get(gv);
+        for (int j = 0; j < K; j++) {
+            row[j] = j < k ? pos[t * k + j] : -1;
+            if (row[j] >= rows_cap) row[j] = -1;
+            wt[j] = w && j < k ? w[t * k + j] : 1.f;
+        }
+        for (int c = of_token * V; c < d; c += threads * V) {
+            Frag<DT, V> g;
+            Frag<YT, V> y[J], o;
+            float gv[V], v[V];
+            g.load(dy + t * lddy + c);
 #pragma unroll
-        for (int j = 0; j < K; j++)
-            if (row[j] >= 0) {
+            for (int j0 = 0; j0 < K; j0 += J) {
+                if (dw)
 #pragma unroll
-                for (int i = 0; i < V; i++) v[i] = wt[j] * gv[i];
-                o.set(v);
-                o.store(dys + (int64_t)row[j] * lddys + c);
-                if (dw) {
-                    y[j].get(v);
+                    for (int j = 0; j < J; j++)
+                        if (row[j0 + j] >= 0) y[j].load(ys + (int64_t)row[j0 + j] * ldys + c);
+                g.get(gv);
 #pragma unroll
-                    for (int i = 0; i < V; i++) dot[j] = fmaf(gv[i], v[i], dot[j]);
-                }
+                for (int j = 0; j < J; j++)
+                    if (row[j0 + j] >= 0) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) v[i] = wt[j0 + j] * gv[i];
+                        o.set(v);
+                        o.store(dys + (int64_t)row[j0 + j] * lddys + c);
+                        if (dw) {
+                            y[j].get(v);
+#pragma unroll
+                            for (int i = 0; i < V; i++) dot[j0 + j] = fmaf(gv[i], v[i], dot[j0 + j]);
+                        }
+                    }
             }
+        }
     }
     if (!dw) return;
 #pragma unroll
@@ -335,11 +374,12 @@ unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict_
         for (int m = 16; m >= 1; m >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
         if (lane == 0) s_dot[warp][j] = dot[j];
     }
-    __syncthreads();
-    if (threadIdx.x < k) {
+    if (threads > 32) __syncthreads();
+    else __syncwarp();
+    if (t < T && of_token < k) {
         float sum = 0.f;
-        for (int i = 0; i < nw; i++) sum += s_dot[i][threadIdx.x];
-        dw[t * k + threadIdx.x] = sum;
+        for (int i = 0; i < threads / 32; i++) sum += s_dot[warp + i][of_token];
+        dw[t * k + of_token] = sum;
     }
 }
 
@@ -371,8 +411,9 @@ int check_rows(const Rows *const *m, int n, int n_out, const char *fn) {
     return OMOE_OK;
 }
 
-template <int V>
-int64_t row_items(int64_t T, int d) { return T * ((d + kChunk<V> - 1) / kChunk<V>); }
+// Blocks of eight warps for `tokens` rows cut into chunks.
+int64_t row_blocks(int64_t tokens, int d, int chunk) { return (tokens * ceil_div(d, chunk) + 7) / 8; }
+const char kTooMany[] = "the rows need too many blocks";
 
 }  // namespace
 }  // namespace omoe
@@ -396,16 +437,19 @@ int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cud
     if (misaligned(topk_idx_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "topk_idx_dev must be 4-byte aligned");
     const int n = plan->n_tokens * plan->top_k, E = plan->n_experts;  // below 2^31: check_plan
     // a warp takes 64 picks before a second CTA joins, and up to eight CTAs share the rest
-    int warps = ceil_div(n, 64), ctas = 1;
-    while (ctas < kPlanCtasMax && warps > ctas * kPlanWarps) ctas *= 2;
-    warps = warps < 1 ? 1 : warps > kPlanWarps ? kPlanWarps : warps;
+    const int64_t want = ((int64_t)n + 63) / 64;
+    int ctas = 1;
+    while (ctas < kPlanCtasMax && want > ctas * kPlanWarps) ctas *= 2;
+    const int warps = want < 8 ? 8 : want > kPlanWarps ? kPlanWarps : (int)want;  // eight for the experts' sums alone
     const int64_t run = round_up(((int64_t)n + ctas * warps - 1) / (ctas * warps), 32);
-    const size_t smem = sizeof(int32_t) * ((size_t)E * (3 + warps) + 1);
+    const size_t tables = sizeof(int32_t) * ((size_t)E * (5 + warps) + 1);
+    int64_t list = warps * run;  // picks of a CTA; beyond what fits they are scattered one by one
+    if (tables + list * 6 > kPlanSmem) list = 0;
+    const size_t smem = tables + list * 6;
     static PerDeviceOnce once;
     bool *done = once.slot();
     if (!done || !*done) {
-        const size_t most = sizeof(int32_t) * ((size_t)OMOE_SORT_MAX_EXPERTS * (3 + kPlanWarps) + 1);
-        cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
         if (e != cudaSuccess) return ops_launched(e, fn);
         if (done) *done = true;
     }
@@ -423,7 +467,7 @@ int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cud
     cfg.attrs = at;
     cfg.numAttrs = ops_pdl() ? 2 : 1;
     return ops_launched(cudaLaunchKernelEx(&cfg, sort_plan_kernel, topk_idx_dev, n, E, (int)plan->row_align,
-                                           (int)plan->rows_cap, (int)run, plan->pos, plan->perm, plan->counts,
+                                           (int)plan->rows_cap, (int)run, (int)list, plan->pos, plan->perm, plan->counts,
                                            plan->offsets), fn);
 }
 
@@ -439,18 +483,18 @@ int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_
     const bool vec = rows_vector(x) && rows_vector(xs);
     const int slices = pad_slices(plan->row_align), pads = E * slices;
     const int64_t tokens = (int64_t)T + pads;  // a slice of an expert's padding is one more "token"
-    const int64_t blocks = ((vec ? row_items<8>(tokens, d) : row_items<1>(tokens, d)) + 7) / 8;
-    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
-    return ops_launched(by_types(x_dtype, xs_dtype, [&](auto *xt, auto *ot) {
-        using XT = std::remove_pointer_t<decltype(xt)>;
-        using OT = std::remove_pointer_t<decltype(ot)>;
-        auto go = [&](auto kern, int chunk) {
-            return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
-                             static_cast<const XT *>(x_dev), ldx, static_cast<OT *>(xs_dev), ldxs, plan->pos, plan->counts,
-                             plan->offsets, T, plan->top_k, pads, slices, d, ceil_div(d, chunk), (int)plan->rows_cap);
-        };
-        return vec ? go(sort_rows_kernel<XT, OT, 8>, kChunk<8>) : go(sort_rows_kernel<XT, OT, 1>, kChunk<1>);
-    }), fn);
+    return by_chunk(vec, d, [&](auto v, auto u) {
+        constexpr int V = decltype(v)::value, U = decltype(u)::value, C = kChunk<V, U>;
+        const int64_t blocks = row_blocks(tokens, d, C);
+        if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
+        return ops_launched(by_types(x_dtype, xs_dtype, [&](auto *xt, auto *ot) {
+            using XT = std::remove_pointer_t<decltype(xt)>;
+            using OT = std::remove_pointer_t<decltype(ot)>;
+            return launch_ex(sort_rows_kernel<XT, OT, V, U>, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream),
+                             ops_pdl(), static_cast<const XT *>(x_dev), ldx, static_cast<OT *>(xs_dev), ldxs, plan->pos, plan->counts,
+                             plan->offsets, T, plan->top_k, pads, slices, d, ceil_div(d, C), (int)plan->rows_cap);
+        }), fn);
+    });
 }
 
 static int unsort(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32_t ys_dtype, const float *w_dev, void *y_dev,
@@ -463,19 +507,21 @@ static int unsort(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32
     if (misaligned(w_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
     if (T == 0) return ops_ok();
     const bool vec = rows_vector(y) && rows_vector(ys);
-    const int64_t blocks = ((vec ? row_items<8>(T, d) : row_items<1>(T, d)) + 7) / 8;
-    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
-    return ops_launched(by_types(ys_dtype, y_dtype, [&](auto *xt, auto *ot) {
-        using XT = std::remove_pointer_t<decltype(xt)>;
-        using OT = std::remove_pointer_t<decltype(ot)>;
-        auto go = [&](auto kern, int chunk) {
-            return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
-                             static_cast<const XT *>(ys_dev), ldys, static_cast<OT *>(y_dev), ldy, plan->pos, w_dev, T,
-                             plan->top_k, d, ceil_div(d, chunk), (int)plan->rows_cap);
-        };
-        if (vec) return w_dev ? go(unsort_rows_kernel<XT, OT, 8, true>, kChunk<8>) : go(unsort_rows_kernel<XT, OT, 8, false>, kChunk<8>);
-        return w_dev ? go(unsort_rows_kernel<XT, OT, 1, true>, kChunk<1>) : go(unsort_rows_kernel<XT, OT, 1, false>, kChunk<1>);
-    }), fn);
+    return by_chunk(vec, d, [&](auto v, auto u) {
+        constexpr int V = decltype(v)::value, U = decltype(u)::value, C = kChunk<V, U>;
+        const int64_t blocks = row_blocks(T, d, C);
+        if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
+        return ops_launched(by_types(ys_dtype, y_dtype, [&](auto *xt, auto *ot) {
+            using XT = std::remove_pointer_t<decltype(xt)>;
+            using OT = std::remove_pointer_t<decltype(ot)>;
+            auto go = [&](auto kern) {
+                return launch_ex(kern, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
+                                 static_cast<const XT *>(ys_dev), ldys, static_cast<OT *>(y_dev), ldy, plan->pos, w_dev, T, plan->top_k,
+                                 d, ceil_div(d, C), (int)plan->rows_cap);
+            };
+            return w_dev ? go(unsort_rows_kernel<XT, OT, V, U, true>) : go(unsort_rows_kernel<XT, OT, V, U, false>);
+        }), fn);
+    });
 }
 
 int omoe_sort_rows_backward(const omoe_sort *plan, const void *dxs_dev, int64_t lddxs, int32_t dxs_dtype, void *dx_dev,
@@ -501,25 +547,27 @@ int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t
     if (misaligned(w_dev, 4) || misaligned(dw_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
     if (T == 0) return ops_ok();
     const int slices = pad_slices(plan->row_align);
-    const int64_t blocks = (int64_t)T + E * slices;
-    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, "the rows need too many blocks");
     const bool vec = rows_vector(dys) && rows_vector(dy) && (!dw_dev || rows_vector(ys));
-    const int per = vec ? 8 : 1;
-    int threads = 64;
+    const int per = vec ? 8 : 1, pads = E * slices;
+    int threads = 32;  // per token: two vectors each, up to a block of 512
     while (threads < 512 && threads * per * 2 < d) threads *= 2;
+    const int block = threads < 128 ? 128 : threads;
+    const int64_t blocks = ((int64_t)T + pads + block / threads - 1) / (block / threads);
+    if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
     return ops_launched(by_types(dy_dtype, ys_dtype, [&](auto *dt, auto *yt) {
         using DT = std::remove_pointer_t<decltype(dt)>;
         using YT = std::remove_pointer_t<decltype(yt)>;
         auto go = [&](auto kern) {
-            return launch_ex(kern, dim3((unsigned)blocks), dim3(threads), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
+            return launch_ex(kern, dim3((unsigned)blocks), dim3(block), 0, static_cast<cudaStream_t>(cuda_stream), ops_pdl(),
                              static_cast<const DT *>(dy_dev), lddy, static_cast<const YT *>(ys_dev), ldys,
-                             static_cast<YT *>(dys_dev), lddys, plan->pos, plan->counts, plan->offsets, w_dev, dw_dev, T, k, slices,
-                             d, (int)plan->rows_cap);
+                             static_cast<YT *>(dys_dev), lddys, plan->pos, plan->counts, plan->offsets, w_dev, dw_dev, T, k, pads, slices,
+                             d, (int)plan->rows_cap, threads);
         };
         auto by_k = [&](auto v) {
             constexpr int V = decltype(v)::value;
             if (k <= 2) return go(unsort_bwd_kernel<DT, YT, V, 2>);
             if (k <= 4) return go(unsort_bwd_kernel<DT, YT, V, 4>);
+            if (k <= 6) return go(unsort_bwd_kernel<DT, YT, V, 6>);
             if (k <= 8) return go(unsort_bwd_kernel<DT, YT, V, 8>);
             return go(unsort_bwd_kernel<DT, YT, V, 16>);
         };

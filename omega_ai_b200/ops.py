@@ -8,6 +8,7 @@ takes from the caching allocator, so calls on different streams and captured gra
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -42,14 +43,14 @@ def _matrix(t: torch.Tensor, rows: int, d: int, name: str, device) -> int:
     """Leading dimension of a [rows, d] matrix on ``device``."""
     if t.shape != (rows, d) or t.device != device:
         _bad(f"{name}: expected [{rows}, {d}] on {device}, got {list(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return d
     ld, one = t.stride()
     if one != 1 and d > 1:
         _bad(f"{name}: the elements of a row must be contiguous")
-    if rows <= 1:
-        return d
-    if ld < d:
+    if rows > 1 and ld < d:
         _bad(f"{name}: rows overlap")
-    return ld
+    return ld if rows > 1 else d
 
 
 def _vector(t, n: int, name: str, device, dtype=torch.float32):
@@ -141,6 +142,14 @@ class TokenSort:
         return out, dw
 
 
+@functools.lru_cache(maxsize=None)
+def _norm_workspace(T: int, d: int) -> int:
+    size = native.lib().omoe_layer_norm_backward_workspace(T, d)
+    if size < 0:
+        _bad(f"x: no rows of width {d}")
+    return size
+
+
 def layer_norm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=None, dtype=None, stats: bool = False):
     """(x - mean) * rstd * gamma + beta per row of x [T, d]; gamma and beta [d] fp32, None for 1 and 0.  With ``stats``
     (y, mean, rstd), which :func:`layer_norm_backward` takes."""
@@ -154,7 +163,8 @@ def layer_norm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=No
     ldo = _matrix(out, T, d, "out", dev)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty(T, dtype=torch.float32, device=dev), torch.empty(T, dtype=torch.float32, device=dev)
+        mean = torch.empty(T, dtype=torch.float32, device=dev)
+        rstd = torch.empty_like(mean)
     _call(dev, native.lib().omoe_layer_norm, x.data_ptr(), ldx, _dt(x.dtype), _vector(gamma, d, "gamma", dev),
           _vector(beta, d, "beta", dev), eps, out.data_ptr(), ldo, _dt(out.dtype), mean.data_ptr() if stats else None,
           rstd.data_ptr() if stats else None, T, d)
@@ -175,13 +185,12 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma, mean: torch.Te
     ldo = _matrix(out, T, d, "out", dev)
     if out.dtype != x.dtype:
         _bad("out: must have the type of x")
-    if d == 0:
-        _bad("x: no columns")
+    size = _norm_workspace(T, d)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
     dgamma = dbeta = None
     if param_grads:
-        dgamma, dbeta = torch.empty(2, d, dtype=torch.float32, device=dev)
-    size = L.omoe_layer_norm_backward_workspace(T, d)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        dgamma = torch.empty(d, dtype=torch.float32, device=dev)
+        dbeta = torch.empty_like(dgamma)
     _call(dev, L.omoe_layer_norm_backward, dy.data_ptr(), lddy, _dt(dy.dtype), x.data_ptr(), ldx, _dt(x.dtype),
           _vector(gamma, d, "gamma", dev), _vector(mean, T, "mean", dev), _vector(rstd, T, "rstd", dev), out.data_ptr(), ldo,
           dgamma.data_ptr() if param_grads else None, dbeta.data_ptr() if param_grads else None, T, d, ws.data_ptr(), size)
