@@ -16,7 +16,7 @@ namespace {
 constexpr int64_t kRowsMax = 0x7fff0000;  // row numbers, and a block's worth beyond them, fit 32 bits
 constexpr int kPlanWarps = 32;
 constexpr int kPlanBatch = 8;    // picks a lane loads together
-constexpr int kPlanCtasMax = 8;  // the portable cluster size
+constexpr int kPlanCtasMax = 16;  // the largest cluster; 8 where the device cannot hold one of 16
 constexpr size_t kPlanSmem = 220 * 1024;
 static_assert(sizeof(int32_t) * (OMOE_SORT_MAX_EXPERTS * (5 + kPlanWarps) + 1) <= kPlanSmem, "the tables of the most experts fit");
 
@@ -67,8 +67,8 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
             if (i0 + u * 32 >= hi) break;
             uint32_t same = 0xffffffffu;  // lanes with this lane's key
             for (int b = 0; b < bits; b++) {
-                const uint32_t set = __ballot_sync(0xffffffffu, (key[u] >> b) & 1);
-                same &= (key[u] >> b) & 1 ? set : ~set;
+                const int bit = (int)((uint32_t)key[u] << (31 - b)) >> 31;  // 0 or all ones
+                same &= ~(__ballot_sync(0xffffffffu, bit) ^ (uint32_t)bit);
             }
             const uint32_t before = same & ((1u << lane) - 1);
             rank[u] = 0;
@@ -411,6 +411,37 @@ int check_rows(const Rows *const *m, int n, int n_out, const char *fn) {
     return OMOE_OK;
 }
 
+// The CTAs of the largest cluster that the current device can hold with all of kPlanSmem, asked once per device.
+cudaError_t plan_ctas(int *most) {
+    static int known[kMaxDevices] = {};  // the same value whoever writes it
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices && known[dev]) {
+        *most = known[dev];
+        return cudaSuccess;
+    }
+    e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kPlanCtasMax);
+    cfg.blockDim = dim3(kPlanWarps * 32);
+    cfg.dynamicSmemBytes = kPlanSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = kPlanCtasMax;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    e = cudaOccupancyMaxActiveClusters(&clusters, sort_plan_kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    *most = clusters > 0 ? kPlanCtasMax : 8;
+    if (dev < kMaxDevices) known[dev] = *most;
+    return cudaSuccess;
+}
+
 // Blocks of eight warps for `tokens` rows cut into chunks.
 int64_t row_blocks(int64_t tokens, int d, int chunk) { return (tokens * ceil_div(d, chunk) + 7) / 8; }
 const char kTooMany[] = "the rows need too many blocks";
@@ -436,23 +467,18 @@ int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cud
     if (plan->n_tokens > 0 && !topk_idx_dev) return ops_fail(OMOE_ERR_INVALID, fn, "null buffer");
     if (misaligned(topk_idx_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "topk_idx_dev must be 4-byte aligned");
     const int n = plan->n_tokens * plan->top_k, E = plan->n_experts;  // below 2^31: check_plan
-    // a warp takes 64 picks before a second CTA joins, and up to eight CTAs share the rest
+    int most = 0;  // CTAs of a cluster
+    if (cudaError_t e = plan_ctas(&most)) return ops_launched(e, fn);
+    // a warp takes 64 picks before a second CTA joins; the CTAs of the largest cluster share the rest
     const int64_t want = ((int64_t)n + 63) / 64;
     int ctas = 1;
-    while (ctas < kPlanCtasMax && want > ctas * kPlanWarps) ctas *= 2;
+    while (ctas < most && want > ctas * kPlanWarps) ctas *= 2;
     const int warps = want < 8 ? 8 : want > kPlanWarps ? kPlanWarps : (int)want;  // eight for the experts' sums alone
     const int64_t run = round_up(((int64_t)n + ctas * warps - 1) / (ctas * warps), 32);
     const size_t tables = sizeof(int32_t) * ((size_t)E * (5 + warps) + 1);
     int64_t list = warps * run;  // picks of a CTA; beyond what fits they are scattered one by one
     if (tables + list * 6 > kPlanSmem) list = 0;
     const size_t smem = tables + list * 6;
-    static PerDeviceOnce once;
-    bool *done = once.slot();
-    if (!done || !*done) {
-        cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
-        if (e != cudaSuccess) return ops_launched(e, fn);
-        if (done) *done = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(warps * 32);
