@@ -28,8 +28,10 @@ __device__ __forceinline__ float block_sum(float v, float *s) {
     return sum;
 }
 
-// Any width: a block walks its row three times, from cache after the first.
-template <typename XT, typename YT>
+// ---- rows of any width ---------------------------------------------------------------------------------------------
+// A block walks its row three times (forward) or twice (backward), from cache after the first; the column sums read everything once
+// more.  What does not fit the registers below, and what those do not have in stages (two fp32 rows of more than 8192).
+template <typename XT, typename YT, int V>
 __global__ void __launch_bounds__(kWideThreads)
 norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta,
                  float eps, YT *__restrict__ y, int64_t ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int d) {
@@ -38,26 +40,47 @@ norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict_
     pdl_trigger();
     pdl_wait();
     const XT *row = x + t * ldx;
-    float sum = 0.f;
-    for (int c = threadIdx.x; c < d; c += kWideThreads) sum += (float)row[c];
+    Frag<XT, V> f;
+    float v[V], sum = 0.f;
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
+        f.load(row + c);
+        f.get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) sum += v[i];
+    }
     const float mean = block_sum(sum, s) / (float)d;
     sum = 0.f;
-    for (int c = threadIdx.x; c < d; c += kWideThreads) {
-        const float v = (float)row[c] - mean;
-        sum = fmaf(v, v, sum);
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
+        f.load(row + c);
+        f.get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) sum = fmaf(v[i] - mean, v[i] - mean, sum);
     }
     const float rstd = rsqrtf(block_sum(sum, s) / (float)d + eps);
     if (threadIdx.x == 0) {
         if (mean_out) mean_out[t] = mean;
         if (rstd_out) rstd_out[t] = rstd;
     }
-    for (int c = threadIdx.x; c < d; c += kWideThreads) {
-        const float h = ((float)row[c] - mean) * rstd;
-        y[t * ldy + c] = (YT)fmaf(h, gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
+    for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
+        Frag<float, V> p;
+        Frag<YT, V> out;
+        float w[V], b[V];
+        f.load(row + c);
+        f.get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) { w[i] = 1.f; b[i] = 0.f; }
+        if (gamma) { p.load_cached(gamma + c); p.get(w); }
+        if (beta) { p.load_cached(beta + c); p.get(b); }
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
+        out.set(v);
+        out.store(y + t * ldy + c);
     }
 }
 
-template <typename XT, typename YT>
+template <typename XT, typename YT, int V>
 __global__ void __launch_bounds__(kWideThreads)
 norm_bwd_wide_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ x, int64_t ldx,
                      const float *__restrict__ gamma, const float *__restrict__ mean, const float *__restrict__ rstd,
@@ -68,56 +91,108 @@ norm_bwd_wide_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restri
     pdl_wait();
     const float m = mean[t], r = rstd[t];
     float sum = 0.f, dot = 0.f;
-    for (int c = threadIdx.x; c < d; c += kWideThreads) {
-        const float g = (float)dy[t * lddy + c] * (gamma ? gamma[c] : 1.f);
-        sum += g;
-        dot = fmaf(g, ((float)x[t * ldx + c] - m) * r, dot);
+    float g[V], h[V];
+    auto take = [&](int c) {  // g = dy * gamma and h of V columns
+        Frag<YT, V> fy;
+        Frag<XT, V> fx;
+        fy.load(dy + t * lddy + c);
+        fx.load(x + t * ldx + c);
+        fy.get(g);
+        fx.get(h);
+        if (gamma) {
+            Frag<float, V> p;
+            float w[V];
+            p.load_cached(gamma + c);
+            p.get(w);
+#pragma unroll
+            for (int i = 0; i < V; i++) g[i] *= w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) h[i] = (h[i] - m) * r;
+    };
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
+        take(c);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            sum += g[i];
+            dot = fmaf(g[i], h[i], dot);
+        }
     }
     const float mg = block_sum(sum, s[0]) / (float)d, mh = block_sum(dot, s[1]) / (float)d;
-    for (int c = threadIdx.x; c < d; c += kWideThreads) {
-        const float g = (float)dy[t * lddy + c] * (gamma ? gamma[c] : 1.f), h = ((float)x[t * ldx + c] - m) * r;
-        dx[t * lddx + c] = (XT)(r * (g - mg - h * mh));
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
+        Frag<XT, V> out;
+        take(c);
+#pragma unroll
+        for (int i = 0; i < V; i++) g[i] = r * (g[i] - mg - h[i] * mh);
+        out.set(g);
+        out.store(dx + t * lddx + c);
     }
 }
 
-// Column sums of a slice of the rows: partial[slice][0][d] of dy * h, [1][d] of dy.
-template <typename XT, typename YT>
+// Column sums of a slice of the rows: partial[slice][0][d] of dy * h, [1][d] of dy.  A warp takes every eighth row of 32 V columns.
+template <typename XT, typename YT, int V>
 __global__ void __launch_bounds__(256)
 norm_cols_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ x, int64_t ldx,
                  const float *__restrict__ mean, const float *__restrict__ rstd, float *__restrict__ partial, int T, int d,
                  int slice) {
-    __shared__ float s[2][8][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    __shared__ float s[2][8][32 * V + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * 32 * V, c = c0 + lane * V;
     pdl_trigger();
     pdl_wait();
     const int64_t t0 = (int64_t)blockIdx.y * slice, t1 = min((int64_t)T, t0 + slice);
-    float a = 0.f, b = 0.f;
-    if (c < d)
+    float a[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) a[i] = b[i] = 0.f;
+    if (c < d) {
+#pragma unroll 4
         for (int64_t t = t0 + warp; t < t1; t += 8) {
-            const float g = (float)dy[t * lddy + c];
-            a = fmaf(g, ((float)x[t * ldx + c] - mean[t]) * rstd[t], a);
-            b += g;
+            Frag<YT, V> fy;
+            Frag<XT, V> fx;
+            float g[V], h[V];
+            fy.load(dy + t * lddy + c);
+            fx.load(x + t * ldx + c);
+            fy.get(g);
+            fx.get(h);
+            const float m = mean[t], r = rstd[t];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                a[i] = fmaf(g[i], (h[i] - m) * r, a[i]);
+                b[i] += g[i];
+            }
         }
-    s[0][warp][lane] = a;
-    s[1][warp][lane] = b;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        s[0][warp][lane * V + i] = a[i];
+        s[1][warp][lane * V + i] = b[i];
+    }
     __syncthreads();
-    if (warp < 2 && c < d) {
+    for (int i = threadIdx.x; i < 64 * V; i += 256) {
+        const int which = i / (32 * V), col = i % (32 * V);
+        if (c0 + col >= d) continue;
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) sum += s[warp][i][lane];
-        partial[((int64_t)blockIdx.y * 2 + warp) * d + c] = sum;
+        for (int w = 0; w < 8; w++) sum += s[which][w][col];
+        partial[((int64_t)blockIdx.y * 2 + which) * d + c0 + col] = sum;
     }
 }
 
 // ---- rows that fit a block's registers ----------------------------------------------------------------------------
 //
-// A block of 512 threads works on 512 / G rows at a time: G threads hold a row, P vectors of V elements each, and walk
-// the rows of the grid with a stride.  Rows arrive in a ring of S stages in shared memory by asynchronous copies that a warp makes for
+// A block of B threads works on B / G rows at a time: G threads hold a row, P vectors of V elements each, and walk the rows of the
+// grid with a stride.  Rows arrive in a ring of S stages in shared memory by asynchronous copies that a warp makes for
 // its own columns alone, so the ring needs no block barrier, and the loads of the next S - 1 rows are on their way while a
 // row is reduced.  The reductions are what threads of a row meet for: warp shuffles, then one named barrier each.
 // Bound by the issue of instructions before it is by HBM, hence pairs of values in the packed fp32 instructions, sums that
 // share their shuffles, and no divisions.
-constexpr int kBlock = 512;
+template <int G>
+constexpr int kFwdBlock = G > 512 ? G : 512;
+// Backward one block per SM leaves half the column sums to join that two do (16384 x 4096 of bf16 73 us against 76, x 1544 of fp32 57
+// against 62); but long rows of fp32 are faster in two (109 us against 121), and 16 rows at a time would run out of barriers.
+template <typename XT, int V, int G, int P>
+constexpr int kBwdBlock = G == 1024 || (V == 8 && P == 1 && G != 64 && !(G == 512 && sizeof(XT) == 4)) ? 1024 : 512;
 
 // Two fp32 values in one register pair.
 typedef unsigned long long f2;
@@ -166,10 +241,10 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
 // piece of bf16 and two of fp32; there pieces 8 .. 15 of every 16 are swapped in pairs, so that eight lanes reading their first
 // pieces meet all banks.
 // V = 1 (rows that are not aligned): one row ahead, in registers.
-template <typename T, int V, int G, int P, int S>
+template <typename T, int B, int V, int G, int P, int S>
 struct Ahead {
     static constexpr int kPieces = sizeof(T) / 2;  // of a thread's vector
-    static constexpr int kVector = kBlock * 16 * kPieces, kStage = kVector * P;
+    static constexpr int kVector = B * 16 * kPieces, kStage = kVector * P;
     uint32_t first, second, put;  // this thread's pieces, and where it puts what it copies
     int col;                      // the first column it copies
     // vectors behind the row's end are zeros in every stage from the start
@@ -216,8 +291,8 @@ struct Ahead {
         }
     }
 };
-template <typename T, int G, int P, int S>
-struct Ahead<T, 1, G, P, S> {
+template <typename T, int B, int G, int P, int S>
+struct Ahead<T, B, 1, G, P, S> {
     static constexpr int kStage = 0;
     Frag<T, 1> next[P];
     __device__ __forceinline__ Ahead(uint32_t, int) {
@@ -250,12 +325,11 @@ struct Part {
     __device__ __forceinline__ int in_row() const { return threadIdx.x % G; }
     __device__ __forceinline__ int col(int q) const { return V == 8 ? (q * G + in_row()) * 8 : in_row(); }
     __device__ __forceinline__ bool has(int q) const { return col(q) < d; }
-    // zeros in place of what lies behind the row's end
+    // single elements: zeros in place of what lies behind the row's end
     __device__ __forceinline__ void mask(int q, f2 (&v)[kPairs]) const {
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {
-            if constexpr (V == 8) v[i] = has(q) ? v[i] : 0ull;
-            else {
+            if constexpr (V == 1) {
                 float a, b;
                 unpack2(v[i], a, b);
                 v[i] = pack2(in_row() + 2 * i * G < d ? a : 0.f, in_row() + (2 * i + 1) * G < d ? b : 0.f);
@@ -297,29 +371,36 @@ struct Part {
     }
 };
 
-// Stages that fit a block's share of shared memory, where `blocks` of them share an SM.
-constexpr int stages(int stage_bytes, int blocks) {
-    const int fit = stage_bytes ? 212992 / blocks / stage_bytes : 2;
-    return fit > 6 ? 6 : fit;
-}
-// two blocks per SM, or one where that leaves fewer than three stages
-template <typename XT, int V, int P>
-constexpr int kFwdStages = V == 1 ? 2 : stages(kBlock * P * V * (int)sizeof(XT), kBlock * P * V * sizeof(XT) * 6 <= 212992 ? 2 : 1);
-// blocks per SM: what the registers and the stages allow
-template <int P>
-constexpr int kBwdBlocks = P == 1 ? 2 : 1;
-template <typename XT, typename YT, int V, int P>
-constexpr int kBwdStages = V == 1 ? 2 : stages(kBlock * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<P>);
-
+// Blocks that share an SM: what the registers allow.
 template <int G>
+constexpr int kFwdBlocks = 1024 / kFwdBlock<G>;
+template <typename XT, int V, int G, int P>
+constexpr int kBwdBlocks = P > 4 || (V == 8 && P > 1) ? 1 : 1024 / kBwdBlock<XT, V, G, P>;
+// Rows that a forward block's threads take at a time.  Where many threads share a row of bf16, two rows share their barriers and
+// shuffles and the loads of gamma and beta; fp32 and narrower rows are faster one by one.
+template <typename XT, int V, int G>
+constexpr int kFwdRows = V == 8 && G >= 512 && sizeof(XT) == 2 ? 2 : 1;
+// Stages that fit a block's share of shared memory: four, six where two long rows are at work (16384 x 4096 of bf16 forward 47.7 us
+// with four and 51.0 with six, 4096 x 16384 66.7 and 58.2).
+constexpr int stages(int stage_bytes, int blocks, int most) {
+    const int fit = stage_bytes ? 212992 / blocks / stage_bytes : 2;
+    return fit > most ? most : fit;
+}
+template <typename XT, int V, int G, int P>
+constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, P > 1 ? 2 + 2 * kFwdRows<XT, V, G> : 4);
+template <typename XT, typename YT, int V, int G, int P>
+constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>, 4);
+
+template <int B, int G>
 __device__ __forceinline__ void row_barrier() {
-    if constexpr (G == kBlock) __syncthreads();
+    static_assert(B == G || G == 32 || B / G < 16, "a named barrier for every row");
+    if constexpr (G == B) __syncthreads();
     else asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / G + 1), "n"(G) : "memory");
 }
 
 // The sum of v over the G threads of a row, in all of them.  s: G / 32 words of this row; between two uses the
 // threads of the row have to meet at another barrier.
-template <int G>
+template <int B, int G>
 __device__ __forceinline__ float row_sum(float v, float *s) {
     constexpr int W = G / 32;
 #pragma unroll
@@ -327,7 +408,7 @@ __device__ __forceinline__ float row_sum(float v, float *s) {
     if constexpr (W > 1) {
         const int lane = threadIdx.x & 31;
         if (lane == 0) s[(threadIdx.x % G) >> 5] = v;
-        row_barrier<G>();
+        row_barrier<B, G>();
         v = s[lane & (W - 1)];
 #pragma unroll
         for (int m = W / 2; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
@@ -336,7 +417,7 @@ __device__ __forceinline__ float row_sum(float v, float *s) {
 }
 
 // Two sums at once, 2 * (G / 32) words: after one exchange the lower half of a warp adds up a and the upper half b.
-template <int G>
+template <int B, int G>
 __device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
     constexpr int W = G / 32;
     const int lane = threadIdx.x & 31, half = lane >> 4;
@@ -346,10 +427,11 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
     for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     if constexpr (W > 1) {
         if ((lane & 15) == 0) s[half * W + ((threadIdx.x % G) >> 5)] = v;
-        row_barrier<G>();
-        v = s[half * W + (lane & (W - 1))];
+        row_barrier<B, G>();
+        v = s[half * W + (lane & (W - 1) & 15)];
+        if constexpr (W == 32) v += s[half * W + 16 + (lane & 15)];
 #pragma unroll
-        for (int m = W / 2; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+        for (int m = W / 2 > 8 ? 8 : W / 2; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     }
     a = __shfl_sync(0xffffffffu, v, 0);
     b = __shfl_sync(0xffffffffu, v, 16);
@@ -377,68 +459,98 @@ struct Param {
 };
 
 template <typename XT, typename YT, int V, int G, int P>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(kFwdBlock<G>, kFwdBlocks<G>)
 norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
             YT *__restrict__ y, int ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
     using Mine = Part<V, G, P>;
-    constexpr int S = kFwdStages<XT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
-    static_assert(S >= 2, "a row is read from one stage while another one fills");
+    constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G>, Q = Mine::kGroups, N = Mine::kPairs;
+    static_assert(S >= 2 * R, "rows are read from some stages while others fill");
     extern __shared__ __align__(16) char sm[];
-    __shared__ float s_sum[2][kBlock / 32];
+    __shared__ float s_sum[2][2 * B / 32];
     const int group = threadIdx.x / G;
-    const int step = gridDim.x * (kBlock / G);
+    const int step = gridDim.x * (B / G);
     const Mine part = {d};
-    Ahead<XT, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d);
+    Ahead<XT, B, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d);
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
     const Param<V, G, P> scale(gamma, part, 1.f), shift(beta, part, 0.f);
-    int t = blockIdx.x * (kBlock / G) + group;  // rows of the grid's stride: T + step stays below 2^31, see the launch
-    int next = t;
-    auto fetch = [&](int stage) {
-        if (next < T) ahead.fetch(stage, x + (int64_t)next * ldx, d);
+    int t = blockIdx.x * (B / G) + group;  // T and the rows of 2 S strides stay below 2^31: kRowsMax
+    int next = t, fill = 0;                        // the row to fetch and its stage
+    auto fetch = [&]() {
+        if (next < T) ahead.fetch(fill, x + (int64_t)next * ldx, d);
         copies_commit();
         next += step;
+        fill = fill + 1 == S ? 0 : fill + 1;
     };
 #pragma unroll
-    for (int i = 0; i < S - 1; i++) fetch(i);
-    float *s_mean = s_sum[0] + group * (G / 32), *s_var = s_sum[1] + group * (G / 32);
-    for (int stage = 0; t < T; t += step) {
-        f2 v[Q][N], pair = 0ull;
-        copies_wait<S - 2>();
+    for (int i = 0; i < S - R; i++) fetch();
+    float *s_mean = s_sum[0] + group * (2 * G / 32), *s_var = s_sum[1] + group * (2 * G / 32);
+    for (int stage = 0; t < T; t += R * step) {
+        f2 v[R][Q][N];
+        float sum[2] = {0.f, 0.f}, mean[2], rstd[2];
+        copies_wait<S - 2 * R>();
 #pragma unroll
-        for (int q = 0; q < Q; q++) ahead.take(stage, q, v[q]);
-        fetch(stage == 0 ? S - 1 : stage - 1);
-        stage = stage + 1 == S ? 0 : stage + 1;
+        for (int r = 0; r < R; r++) {
 #pragma unroll
-        for (int q = 0; q < Q; q++)
-#pragma unroll
-            for (int i = 0; i < N; i++) pair = add2(pair, v[q][i]);
-        const float mean = row_sum<G>(both(pair), s_mean) * inv;
-        const f2 minus = pack2(-mean, -mean);
-        pair = 0ull;
-#pragma unroll
-        for (int q = 0; q < Q; q++) {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[q][i] = add2(v[q][i], minus);
-            part.mask(q, v[q]);
-#pragma unroll
-            for (int i = 0; i < N; i++) pair = fma2(v[q][i], v[q][i], pair);
+            for (int q = 0; q < Q; q++) ahead.take(stage, q, v[r][q]);
+            stage = stage + 1 == S ? 0 : stage + 1;
         }
-        const float rstd = rsqrtf(fmaf(row_sum<G>(both(pair), s_var), inv, eps));
+#pragma unroll
+        for (int r = 0; r < R; r++) fetch();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            f2 pair = 0ull;
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int i = 0; i < N; i++) pair = add2(pair, v[r][q][i]);
+            sum[r] = both(pair);
+        }
+        if constexpr (R == 2) row_sums<B, G>(sum[0], sum[1], s_mean);
+        else sum[0] = row_sum<B, G>(sum[0], s_mean);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            mean[r] = sum[r] * inv;
+            const f2 minus = pack2(-mean[r], -mean[r]);
+            f2 pair = 0ull;
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                if (V == 8 && !part.has(q)) continue;  // a branch: all but one warp of a row go the same way
+#pragma unroll
+                for (int i = 0; i < N; i++) v[r][q][i] = add2(v[r][q][i], minus);
+                part.mask(q, v[r][q]);
+#pragma unroll
+                for (int i = 0; i < N; i++) pair = fma2(v[r][q][i], v[r][q][i], pair);
+            }
+            sum[r] = both(pair);
+        }
+        if constexpr (R == 2) row_sums<B, G>(sum[0], sum[1], s_var);
+        else sum[0] = row_sum<B, G>(sum[0], s_var);
+#pragma unroll
+        for (int r = 0; r < R; r++) rstd[r] = rsqrtf(fmaf(sum[r], inv, eps));
         if (part.in_row() == 0) {
-            if (mean_out) mean_out[t] = mean;
-            if (rstd_out) rstd_out[t] = rstd;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (t + r * step < T) {
+                    if (mean_out) mean_out[t + r * step] = mean[r];
+                    if (rstd_out) rstd_out[t + r * step] = rstd[r];
+                }
         }
-        const f2 r = pack2(rstd, rstd);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             f2 w[N], b[N];
             scale.get(part, q, w);
             shift.get(part, q, b);
 #pragma unroll
-            for (int i = 0; i < N; i++) w[i] = fma2(mul2(v[q][i], r), w[i], b[i]);
-            part.store(y + (int64_t)t * ldy, q, w);
+            for (int r = 0; r < R; r++) {
+                if (t + r * step >= T) break;
+                const f2 rr = pack2(rstd[r], rstd[r]);
+                f2 out[N];
+#pragma unroll
+                for (int i = 0; i < N; i++) out[i] = fma2(mul2(v[r][q][i], rr), w[i], b[i]);
+                part.store(y + (int64_t)(t + r * step) * ldy, q, out);
+            }
         }
     }
 }
@@ -446,18 +558,18 @@ norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, 
 // The column sums of dy * h and dy stay in registers over all of a block's rows; each block leaves them in `partial`.  With
 // several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
 template <typename XT, typename YT, int V, int G, int P>
-__global__ void __launch_bounds__(kBlock, kBwdBlocks<P>)
+__global__ void __launch_bounds__(kBwdBlock<XT, V, G, P>, kBwdBlocks<XT, V, G, P>)
 norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, int ldx, const float *__restrict__ gamma,
                 const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, int lddx,
                 float *__restrict__ partial, int T, int d) {
     using Mine = Part<V, G, P>;
-    constexpr int S = kBwdStages<XT, YT, V, P>, Q = Mine::kGroups, N = Mine::kPairs;
+    constexpr int B = kBwdBlock<XT, V, G, P>, S = kBwdStages<XT, YT, V, G, P>, Q = Mine::kGroups, N = Mine::kPairs;
     constexpr bool kAgain = Q > 1;
     static_assert(S >= 2, "a row is read from one stage while another one fills");
     extern __shared__ __align__(16) char sm[];
-    __shared__ float s_sum[2][2 * kBlock / 32];
+    __shared__ float s_sum[2][2 * B / 32];
     const int group = threadIdx.x / G;
-    const int step = gridDim.x * (kBlock / G);
+    const int step = gridDim.x * (B / G);
     const Mine part = {d};
     f2 dg[Q][N], db[Q][N];
 #pragma unroll
@@ -465,13 +577,13 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
 #pragma unroll
         for (int i = 0; i < N; i++) dg[q][i] = db[q][i] = 0ull;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm);
-    Ahead<XT, V, G, P, S> ahead_x(ring, d);
-    Ahead<YT, V, G, P, S> ahead_y(ring + S * Ahead<XT, V, G, P, S>::kStage, d);
+    Ahead<XT, B, V, G, P, S> ahead_x(ring, d);
+    Ahead<YT, B, V, G, P, S> ahead_y(ring + S * Ahead<XT, B, V, G, P, S>::kStage, d);
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
     const Param<V, G, P> scale(gamma, part, 1.f);
-    int t = blockIdx.x * (kBlock / G) + group, next = t;
+    int t = blockIdx.x * (B / G) + group, next = t;
     auto fetch = [&](int stage) {
         if (next < T) {
             ahead_x.fetch(stage, x + (int64_t)next * ldx, d);
@@ -520,7 +632,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
             }
         }
         float mg = both(sum_g), mh = both(sum_gh);
-        row_sums<G>(mg, mh, s_sum[odd] + group * (2 * G / 32));
+        row_sums<B, G>(mg, mh, s_sum[odd] + group * (2 * G / 32));
         const f2 less = pack2(-mg * inv, -mg * inv), slope = pack2(-mh * inv, -mh * inv);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
@@ -545,7 +657,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
     if (!partial) return;
     // column sums of the block: the rows' groups joined through shared memory, in order
     float *sums = partial + (int64_t)blockIdx.x * 2 * d;
-    if constexpr (G == kBlock) {
+    if constexpr (G == B) {
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             part.store(sums, q, dg[q]);
@@ -567,12 +679,12 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
                 unpack2(db[q][i], b[0], b[next_c]);
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * W; i += kBlock) {
+        for (int i = threadIdx.x; i < 2 * W; i += B) {
             const int which = i / W, col = i % W;
             if (col >= d) continue;
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < kBlock / G; q++) sum += s[(q * 2 + which) * W + col];
+            for (int q = 0; q < B / G; q++) sum += s[(q * 2 + which) * W + col];
             sums[which * d + col] = sum;
         }
     }
@@ -607,11 +719,11 @@ constexpr int kBwdBlocksMax = 320;
 int slices_of(int T) { return T < kSlicesMax ? (T < 1 ? 1 : T) : kSlicesMax; }
 
 // Calls f with the vector width, threads per row and vectors per thread (integral constants) for rows of width d, or
-// returns false where they do not fit a block's registers.  Vectors: the fewest threads that hold the row with one each, then all of the
-// block with more.  Single elements: four per thread.
+// returns false where they do not fit a block's registers.  Vectors: the fewest threads that hold the row with one each, then two.
+// Single elements: four per thread, then eight.
 template <int N>
 using Int = std::integral_constant<int, N>;
-template <typename F>
+template <bool BACK, typename F>
 bool by_width(bool vec, int d, F f) {
     if (vec) {
         if (d <= 256) f(Int<8>(), Int<32>(), Int<1>());
@@ -619,9 +731,12 @@ bool by_width(bool vec, int d, F f) {
         else if (d <= 1024) f(Int<8>(), Int<128>(), Int<1>());
         else if (d <= 2048) f(Int<8>(), Int<256>(), Int<1>());
         else if (d <= 4096) f(Int<8>(), Int<512>(), Int<1>());
-        else if (d <= 8192) f(Int<8>(), Int<512>(), Int<2>());
-        else if (d <= 16384) f(Int<8>(), Int<512>(), Int<4>());
-        else return false;
+        else if (d <= 8192) f(Int<8>(), Int<1024>(), Int<1>());
+        else if (d <= 16384) {
+            // backward, two vectors' column sums spill from 64 registers; four vectors have 128
+            if constexpr (BACK) f(Int<8>(), Int<512>(), Int<4>());
+            else f(Int<8>(), Int<1024>(), Int<2>());
+        } else return false;
     } else {
         if (d <= 128) f(Int<1>(), Int<32>(), Int<4>());
         else if (d <= 512) f(Int<1>(), Int<128>(), Int<4>());
@@ -669,21 +784,25 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
         using XT = std::remove_pointer_t<decltype(xt)>;
         using YT = std::remove_pointer_t<decltype(yt)>;
         cudaError_t e = cudaSuccess;
-        if (by_width(rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 32) && !misaligned(beta_dev, 32), d,
+        const bool vec = rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 32) && !misaligned(beta_dev, 32);
+        if (by_width<false>(vec, d,
                      [&](auto v, auto g, auto p) {
                          constexpr int V = decltype(v)::value, G = decltype(g)::value, P = decltype(p)::value;
-                         constexpr size_t smem = kFwdStages<XT, V, P> * Ahead<XT, V, G, P, 2>::kStage;
+                         constexpr size_t smem = kFwdStages<XT, V, G, P> * Ahead<XT, kFwdBlock<G>, V, G, P, 2>::kStage;
                          static PerDeviceOnce once;
                          e = allow_smem(norm_kernel<XT, YT, V, G, P>, smem, once);
                          if (e != cudaSuccess) return;
-                         const int blocks = ceil_div(T, kBlock / G), most = 2 * sms;
-                         e = launch_ex(norm_kernel<XT, YT, V, G, P>, dim3(blocks < most ? blocks : most), dim3(kBlock), smem, s, ops_pdl(),
+                         const int blocks = ceil_div(T, kFwdBlock<G> / G), most = kFwdBlocks<G> * sms;
+                         e = launch_ex(norm_kernel<XT, YT, V, G, P>, dim3(blocks < most ? blocks : most), dim3(kFwdBlock<G>), smem, s, ops_pdl(),
                                        static_cast<const XT *>(x_dev), (int)ldx, gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev), (int)ldy,
                                        mean_dev, rstd_dev, T, d);
                      }))
             return e;
-        return launch_ex(norm_wide_kernel<XT, YT>, dim3(T), dim3(kWideThreads), 0, s, ops_pdl(), static_cast<const XT *>(x_dev),
-                         ldx, gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev), ldy, mean_dev, rstd_dev, d);
+        auto wide = [&](auto kern) {
+            return launch_ex(kern, dim3(T), dim3(kWideThreads), 0, s, ops_pdl(), static_cast<const XT *>(x_dev), ldx, gamma_dev,
+                             beta_dev, eps, static_cast<YT *>(y_dev), ldy, mean_dev, rstd_dev, d);
+        };
+        return vec ? wide(norm_wide_kernel<XT, YT, 8>) : wide(norm_wide_kernel<XT, YT, 1>);
     }), fn);
 }
 
@@ -722,22 +841,23 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
         const XT *in = static_cast<const XT *>(x_dev);
         cudaError_t e = cudaSuccess;
         int sums = 0;  // column sums in the workspace
-        if (T > 0 && by_width(rows_vector(x) && rows_vector(dy) && rows_vector(dx) && !misaligned(gamma_dev, 32), d,
+        const bool vec = rows_vector(x) && rows_vector(dy) && rows_vector(dx) && !misaligned(gamma_dev, 32);
+        if (T > 0 && by_width<true>(vec, d,
                               [&](auto v, auto gg, auto p) {
                                   constexpr int V = decltype(v)::value, G = decltype(gg)::value, P = decltype(p)::value;
-                                  constexpr int S = kBwdStages<XT, YT, V, P>;
+                                  constexpr int S = kBwdStages<XT, YT, V, G, P>, B = kBwdBlock<XT, V, G, P>;
                                   if constexpr (S >= 2) {
-                                      constexpr size_t ring = S * (Ahead<XT, V, G, P, S>::kStage + Ahead<YT, V, G, P, S>::kStage);
-                                      constexpr size_t join = G < kBlock ? 2 * kBlock * P * V * sizeof(float) : 0;
+                                      constexpr size_t ring = S * (Ahead<XT, B, V, G, P, S>::kStage + Ahead<YT, B, V, G, P, S>::kStage);
+                                      constexpr size_t join = G < B ? 2 * B * P * V * sizeof(float) : 0;
                                       constexpr size_t smem = ring > join ? ring : join;
                                       static PerDeviceOnce once;
                                       e = allow_smem(norm_bwd_kernel<XT, YT, V, G, P>, smem, once);
                                       if (e != cudaSuccess) return;
-                                      const int blocks = ceil_div(T, kBlock / G);
-                                      int most = kBwdBlocks<P> * sms;
+                                      const int blocks = ceil_div(T, B / G);
+                                      int most = kBwdBlocks<XT, V, G, P> * sms;
                                       most = most < kBwdBlocksMax ? most : kBwdBlocksMax;
                                       sums = blocks < most ? blocks : most;
-                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(kBlock), smem, s, ops_pdl(), g, (int)lddy, in,
+                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(B), smem, s, ops_pdl(), g, (int)lddy, in,
                                                     (int)ldx, gamma_dev, mean_dev, rstd_dev, static_cast<XT *>(dx_dev), (int)lddx,
                                                     params ? partial : nullptr, T, d);
                                   }
@@ -745,15 +865,18 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
             if (e != cudaSuccess || !params) return e;
             return launch_ex(norm_join_kernel, dim3(cols, 2), dim3(1024), 0, s, ops_pdl(), partial, sums, d, dgamma_dev, dbeta_dev);
         }
-        if (T > 0) {
-            e = launch_ex(norm_bwd_wide_kernel<XT, YT>, dim3(T), dim3(kWideThreads), 0, s, ops_pdl(), g, lddy, in, ldx, gamma_dev,
-                          mean_dev, rstd_dev, static_cast<XT *>(dx_dev), lddx, d);
+        auto wide = [&](auto kern, auto cols_kern, int V) {
+            cudaError_t e = cudaSuccess;
+            if (T > 0)
+                e = launch_ex(kern, dim3(T), dim3(kWideThreads), 0, s, ops_pdl(), g, lddy, in, ldx, gamma_dev, mean_dev, rstd_dev,
+                              static_cast<XT *>(dx_dev), lddx, d);
             if (e != cudaSuccess || !params) return e;
-        }
-        if (!params) return e;
-        e = launch_ex(norm_cols_kernel<XT, YT>, dim3(cols, slices), dim3(256), 0, s, ops_pdl(), g, lddy, in, ldx, mean_dev,
-                      rstd_dev, partial, T, d, ceil_div(T, slices));
-        if (e != cudaSuccess) return e;
+            return launch_ex(cols_kern, dim3(ceil_div(d, 32 * V), slices), dim3(256), 0, s, ops_pdl(), g, lddy, in, ldx, mean_dev, rstd_dev,
+                             partial, T, d, ceil_div(T, slices));
+        };
+        e = vec ? wide(norm_bwd_wide_kernel<XT, YT, 8>, norm_cols_kernel<XT, YT, 8>, 8)
+                : wide(norm_bwd_wide_kernel<XT, YT, 1>, norm_cols_kernel<XT, YT, 1>, 1);
+        if (e != cudaSuccess || !params) return e;
         return launch_ex(norm_join_kernel, dim3(cols, 2), dim3(1024), 0, s, ops_pdl(), partial, slices, d, dgamma_dev, dbeta_dev);
     }), fn);
 }
