@@ -35,10 +35,14 @@ SYMBOLS = (
     "omoe_set_profiling", "omoe_get_stage_ms", "omoe_get_stage_ms_at", "omoe_ep_export", "omoe_ep_import",
     "omoe_route_noalloc", "omoe_route_noalloc_error",
     "omoe_ep_connect_local", "omoe_set_training", "omoe_backward", "omoe_backward_block", "omoe_get_weight_grads", "omoe_set_aux_loss", "omoe_get_aux_loss",
+)
+# of these the operators without a handle, which ops.py calls through the torch binding
+OPERATORS = (
     "omoe_ops_error", "omoe_sort_rows_cap", "omoe_sort_plan", "omoe_sort_rows", "omoe_sort_rows_backward", "omoe_unsort_rows",
     "omoe_unsort_rows_backward", "omoe_layer_norm", "omoe_layer_norm_backward_workspace", "omoe_layer_norm_backward",
     "omoe_grad_norm", "omoe_grad_scale", "omoe_grad_clip",
 )
+SYMBOLS += OPERATORS
 SORT_MAX_EXPERTS = 1024
 GRAD_WORKSPACE_BYTES = 16384
 NOALLOC_MAX_TOKENS = 4096
@@ -88,6 +92,26 @@ def build(force: bool = False, check: bool = False) -> str:
     stale = (not os.path.exists(path)) or any(os.path.getmtime(s) > os.path.getmtime(path) for s in sources())
     if force or stale:
         subprocess.check_call(["sh", os.path.join(CSRC, "build.sh")] + (["check"] if check else []))
+    if not check:
+        build_binding(force)
+    return path
+
+
+def build_binding(force: bool = False) -> str:
+    """Compile ``_torch_ops.so``, the operators' binding for torch tensors, against the installed torch."""
+    import sysconfig
+
+    import torch
+
+    src, header = os.path.join(CSRC, "bind", "torch_ops.cpp"), os.path.join(os.path.dirname(_PKG), "include", "omoe.h")
+    path = os.path.join(_PKG, "_torch_ops.so")
+    if force or not os.path.exists(path) or any(os.path.getmtime(s) > os.path.getmtime(path) for s in (src, header)):
+        home, cuda = os.path.dirname(torch.__file__), os.environ.get("CUDA_HOME", "/usr/local/cuda")
+        subprocess.check_call(
+            [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
+             f"-I{home}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", src,
+             "-o", path, f"-L{home}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
     return path
 
 
