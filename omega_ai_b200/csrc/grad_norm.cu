@@ -24,13 +24,13 @@ struct Entry {
     int32_t first;  // chunk
     int32_t dtype;
 };
-// As many tensors as one launch takes: few, or what fits the kernel parameters.
+// The tensors of one launch.  A parameter is copied with every launch, 32 KB of them for longer than 16 MB of gradients take; so there
+// are tables of several sizes, the largest what fits the kernel parameters.
 template <int N>
 struct Table {
     Entry e[N];
     int32_t n, chunks;
 };
-constexpr int kFew = 48, kMany = 1000;
 
 // The sum of 16 values' squares.  In fp32 first, with four chains; where that overflows, or is so small that squares
 // have lost digits, again in fp64 (the squares of fp32 values are exact there and their sum stays in range).
@@ -321,6 +321,16 @@ int used(const omoe_tensor *t, int n) {
     return m;
 }
 
+template <typename F>
+cudaError_t by_count(const omoe_tensor *grads, const omoe_tensor *out, int n, int most, F f) {
+    const int m = used(grads, n);
+    if (m <= 16) return tables<16>(grads, out, n, most, f);
+    if (m <= 64) return tables<64>(grads, out, n, most, f);
+    if (m <= 256) return tables<256>(grads, out, n, most, f);
+    if (m <= 500) return tables<500>(grads, out, n, most, f);
+    return tables<1000>(grads, out, n, most, f);
+}
+
 // Blocks' sums of squares into the workspace; *slots is how many there are.
 cudaError_t launch_squares(const omoe_tensor *grads, int n, double *ws, int sms, cudaStream_t s, int *slots) {
     *slots = 0;
@@ -332,8 +342,7 @@ cudaError_t launch_squares(const omoe_tensor *grads, int n, double *ws, int sms,
         const int b = first ? blocks : (blocks < *slots ? blocks : *slots);
         return launch_ex(grad_squares_kernel<N>, dim3(b), dim3(kThreads), 0, s, ops_pdl(), t, ws, first ? 0 : 1);
     };
-    return used(grads, n) <= kFew ? tables<kFew>(grads, nullptr, n, sms * kSumBlocks, go)
-                                   : tables<kMany>(grads, nullptr, n, sms * kSumBlocks, go);
+    return by_count(grads, nullptr, n, sms * kSumBlocks, go);
 }
 
 cudaError_t launch_scale(const omoe_tensor *grads, const omoe_tensor *out, int n, const double *ws, int slots, const float *norm_in,
@@ -344,8 +353,7 @@ cudaError_t launch_scale(const omoe_tensor *grads, const omoe_tensor *out, int n
         return launch_ex(grad_scale_kernel<N>, dim3(blocks), dim3(kThreads), 0, s, ops_pdl(), t, ws, slots, norm_in,
                          first ? norm_out : nullptr, max_norm, out ? 0 : 1);
     };
-    return used(grads, n) <= kFew ? tables<kFew>(grads, out, n, sms * kScaleBlocks, go)
-                                   : tables<kMany>(grads, out, n, sms * kScaleBlocks, go);
+    return by_count(grads, out, n, sms * kScaleBlocks, go);
 }
 
 const char *norm_args_wrong(const float *norm, const void *ws, int64_t bytes) {

@@ -235,13 +235,14 @@ sort_rows_kernel(const XT *__restrict__ x, int64_t ldx, OT *__restrict__ xs, int
         return;
     }
     const int r = pick_row(pos, t, k, lane, rows_cap);
-    uint32_t picks = __ballot_sync(0xffffffffu, r >= 0);
-    if (!picks) return;
     Frag<XT, V> in[U];
     Frag<OT, V> out[U];
+    // before the picks are there: a token that turns out to have none was read for nothing, the others have waited once, not twice
 #pragma unroll
     for (int u = 0; u < U; u++)
         if (c0 + u * 32 * V < d) in[u].load(x + t * ldx + c0 + u * 32 * V);
+    uint32_t picks = __ballot_sync(0xffffffffu, r >= 0);
+    if (!picks) return;
 #pragma unroll
     for (int u = 0; u < U; u++) convert(in[u], out[u]);
     for (; picks; picks &= picks - 1) {
