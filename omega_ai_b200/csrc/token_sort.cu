@@ -173,18 +173,20 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     if (ctas > 1) cluster.sync();  // the others may still read this CTA's totals
 }
 
-// A warp takes one chunk of a token's columns: U vectors per lane.  Narrow rows get fewer (a warp that has nothing to do for most of
-// its vectors still issues for them: 20 us against 11 for 16384 tokens of 128 columns and 8 picks).
+// A warp takes one chunk of a token's columns: U vectors per lane.  Rows of up to 256 columns get one (a warp that has nothing to do for
+// most of its vectors still issues for them: 20 us against 10 for the way back of 16384 x 128 and 8 picks).  Else two; sums over picks
+// four where those chunks fill the GPU's warps by themselves (16384 x 4096, 2 picks: 65 us against 71; 4096 x 1024: 5.5 against 5.4).
 template <int V, int U>
 constexpr int kChunk = 32 * V * U;
-// Calls f(V, U) (integral constants) for rows of width d.
+// Calls f(V, U) (integral constants) for T rows of width d.
 template <typename F>
-int by_chunk(bool vec, int d, F f) {
+int by_chunk(bool vec, int64_t T, int d, bool sums, F f) {
     using std::integral_constant;
     if (!vec) return f(integral_constant<int, 1>(), integral_constant<int, 8>());
     if (d <= 256) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
-    if (d <= 512) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
-    return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+    if (sums && T * ceil_div(d, kChunk<8, 4>) > (int64_t)64 * ops_sm_count())
+        return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+    return f(integral_constant<int, 8>(), integral_constant<int, 2>());
 }
 
 // The rows of a token's picks, a pick per lane; picks without a row, or with one that no plan makes, are negative.
@@ -321,6 +323,7 @@ unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict_
                   int64_t lddys, const int32_t *__restrict__ pos, const int32_t *__restrict__ counts,
                   const int32_t *__restrict__ offsets, const float *__restrict__ w, float *__restrict__ dw, int T, int k, int pads,
                   int slices, int d, int rows_cap, int threads) {
+    constexpr int U = V > 1 ? 1 : K <= 4 ? 4 : 2;  // single elements: several columns' loads together
     constexpr int J = K <= 6 || (sizeof(YT) * V <= 16 && K <= 8) ? K : 4;  // picks whose vectors are held at a time
     __shared__ float s_dot[16][K];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, of_token = threadIdx.x % threads;
@@ -340,31 +343,41 @@ unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict_
             if (row[j] >= rows_cap) row[j] = -1;
             wt[j] = w && j < k ? w[t * k + j] : 1.f;
         }
-        for (int c = of_token * V; c < d; c += threads * V) {
-            Frag<DT, V> g;
-            Frag<YT, V> y[J], o;
+        for (int c0 = of_token * V; c0 < d; c0 += threads * V * U) {
+            Frag<DT, V> g[U];
+            Frag<YT, V> y[U][J], o;
             float gv[V], v[V];
-            g.load(dy + t * lddy + c);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (c0 + u * threads * V < d) g[u].load(dy + t * lddy + c0 + u * threads * V);
 #pragma unroll
             for (int j0 = 0; j0 < K; j0 += J) {
                 if (dw)
 #pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int j = 0; j < J; j++)
+                            if (row[j0 + j] >= 0 && c0 + u * threads * V < d)
+                                y[u][j].load(ys + (int64_t)row[j0 + j] * ldys + c0 + u * threads * V);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int c = c0 + u * threads * V;
+                    if (U > 1 && c >= d) break;
+                    g[u].get(gv);
+#pragma unroll
                     for (int j = 0; j < J; j++)
-                        if (row[j0 + j] >= 0) y[j].load(ys + (int64_t)row[j0 + j] * ldys + c);
-                g.get(gv);
+                        if (row[j0 + j] >= 0) {
 #pragma unroll
-                for (int j = 0; j < J; j++)
-                    if (row[j0 + j] >= 0) {
+                            for (int i = 0; i < V; i++) v[i] = wt[j0 + j] * gv[i];
+                            o.set(v);
+                            o.store(dys + (int64_t)row[j0 + j] * lddys + c);
+                            if (dw) {
+                                y[u][j].get(v);
 #pragma unroll
-                        for (int i = 0; i < V; i++) v[i] = wt[j0 + j] * gv[i];
-                        o.set(v);
-                        o.store(dys + (int64_t)row[j0 + j] * lddys + c);
-                        if (dw) {
-                            y[j].get(v);
-#pragma unroll
-                            for (int i = 0; i < V; i++) dot[j0 + j] = fmaf(gv[i], v[i], dot[j0 + j]);
+                                for (int i = 0; i < V; i++) dot[j0 + j] = fmaf(gv[i], v[i], dot[j0 + j]);
+                            }
                         }
-                    }
+                }
             }
         }
     }
@@ -510,7 +523,7 @@ int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_
     const bool vec = rows_vector(x) && rows_vector(xs);
     const int slices = pad_slices(plan->row_align), pads = E * slices;
     const int64_t tokens = (int64_t)T + pads;  // a slice of an expert's padding is one more "token"
-    return by_chunk(vec, d, [&](auto v, auto u) {
+    return by_chunk(vec, T, d, false, [&](auto v, auto u) {
         constexpr int V = decltype(v)::value, U = decltype(u)::value, C = kChunk<V, U>;
         const int64_t blocks = row_blocks(tokens, d, C);
         if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
@@ -534,7 +547,7 @@ static int unsort(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32
     if (misaligned(w_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
     if (T == 0) return ops_ok();
     const bool vec = rows_vector(y) && rows_vector(ys);
-    return by_chunk(vec, d, [&](auto v, auto u) {
+    return by_chunk(vec, T, d, true, [&](auto v, auto u) {
         constexpr int V = decltype(v)::value, U = decltype(u)::value, C = kChunk<V, U>;
         const int64_t blocks = row_blocks(T, d, C);
         if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
@@ -575,9 +588,9 @@ int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t
     if (T == 0) return ops_ok();
     const int slices = pad_slices(plan->row_align);
     const bool vec = rows_vector(dys) && rows_vector(dy) && (!dw_dev || rows_vector(ys));
-    const int per = vec ? 8 : 1, pads = E * slices;
-    int threads = 32;  // per token: two vectors each, up to a block of 512
-    while (threads < 512 && threads * per * 2 < d) threads *= 2;
+    const int pads = E * slices;
+    int threads = 32;  // per token: two vectors or eight elements each, up to a block of 512
+    while (threads < 512 && threads * (vec ? 16 : 8) < d) threads *= 2;
     const int block = threads < 128 ? 128 : threads;
     const int64_t blocks = ((int64_t)T + pads + block / threads - 1) / (block / threads);
     if (blocks > INT32_MAX) return ops_fail(OMOE_ERR_TOO_LARGE, fn, kTooMany);
