@@ -356,8 +356,22 @@ cudaError_t launch_scale(const omoe_tensor *grads, const omoe_tensor *out, int n
     return by_count(grads, out, n, sms * kScaleBlocks, go);
 }
 
+// True where [p, p + bytes) meets a tensor of the lists.
+bool meets(const void *p, size_t bytes, const omoe_tensor *grads, const omoe_tensor *out, int n) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p), hi = lo + bytes;
+    for (int i = 0; i < n; i++) {
+        const uintptr_t size = (uintptr_t)grads[i].count * (grads[i].dtype == OMOE_BF16 ? 2 : 4);
+        const uintptr_t a = reinterpret_cast<uintptr_t>(grads[i].ptr), b = out ? reinterpret_cast<uintptr_t>(out[i].ptr) : a;
+        if (size && ((a < hi && lo < a + size) || (b < hi && lo < b + size))) return true;
+    }
+    return false;
+}
+const char kMeets[] = "norm_dev or the workspace overlaps a tensor of the list";
+
 const char *norm_args_wrong(const float *norm, const void *ws, int64_t bytes) {
     if (!norm || misaligned(norm, 4)) return "norm_dev is null or misaligned";
+    const uintptr_t at = reinterpret_cast<uintptr_t>(norm), w = reinterpret_cast<uintptr_t>(ws);
+    if (ws && at + 4 > w && at < w + OMOE_GRAD_WORKSPACE_BYTES) return "norm_dev lies in the workspace";
     if (!ws || misaligned(ws, 16) || bytes < OMOE_GRAD_WORKSPACE_BYTES) return "the workspace is missing, misaligned or too small";
     return nullptr;
 }
@@ -374,6 +388,8 @@ int omoe_grad_norm(const omoe_tensor *grads, int32_t n, float *norm_dev, void *w
     const char *fn = "omoe_grad_norm";
     if (int rc = check_list(grads, nullptr, n, false, fn)) return rc;
     if (const char *bad = norm_args_wrong(norm_dev, workspace_dev, workspace_bytes)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
+    if (meets(norm_dev, 4, grads, nullptr, n) || meets(workspace_dev, OMOE_GRAD_WORKSPACE_BYTES, grads, nullptr, n))
+        return ops_fail(OMOE_ERR_INVALID, fn, kMeets);
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
@@ -390,6 +406,7 @@ int omoe_grad_scale(const omoe_tensor *grads, const omoe_tensor *out, int32_t n,
     if (int rc = check_list(grads, out, n, true, fn)) return rc;
     if (!norm_dev || misaligned(norm_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "norm_dev is null or misaligned");
     if (!(max_norm >= 0.f)) return ops_fail(OMOE_ERR_INVALID, fn, "max_norm must not be negative");
+    if (meets(norm_dev, 4, grads, out, n)) return ops_fail(OMOE_ERR_INVALID, fn, kMeets);
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
     return ops_launched(launch_scale(grads, out, n, nullptr, 0, norm_dev, nullptr, max_norm, sms, static_cast<cudaStream_t>(cuda_stream)), fn);
@@ -401,6 +418,8 @@ int omoe_grad_clip(const omoe_tensor *grads, const omoe_tensor *out, int32_t n, 
     if (int rc = check_list(grads, out, n, true, fn)) return rc;
     if (const char *bad = norm_args_wrong(norm_dev, workspace_dev, workspace_bytes)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
     if (!(max_norm >= 0.f)) return ops_fail(OMOE_ERR_INVALID, fn, "max_norm must not be negative");
+    if (meets(norm_dev, 4, grads, out, n) || meets(workspace_dev, OMOE_GRAD_WORKSPACE_BYTES, grads, out, n))
+        return ops_fail(OMOE_ERR_INVALID, fn, kMeets);
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);

@@ -773,9 +773,10 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
     const Rows x = {x_dev, ldx, x_dtype, T, d}, y = {y_dev, ldy, y_dtype, T, d};
     if (const char *bad = rows_wrong(x)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
     if (const char *bad = rows_wrong(y)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
-    if (rows_overlap(y, x)) return ops_fail(OMOE_ERR_INVALID, fn, "an output overlaps another buffer");
     if (misaligned(gamma_dev, 4) || misaligned(beta_dev, 4) || misaligned(mean_dev, 4) || misaligned(rstd_dev, 4))
         return ops_fail(OMOE_ERR_INVALID, fn, "fp32 buffers must be 4-byte aligned");
+    const Rows all[] = {y, words(mean_dev, T), words(rstd_dev, T), x, words(gamma_dev, d), words(beta_dev, d)};
+    if (int rc = ops_apart(all, 6, 3, fn)) return rc;
     if (T == 0) return ops_ok();
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
@@ -821,13 +822,15 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
     const Rows dx = {dx_dev, lddx, x_dtype, T, d}, dy = {dy_dev, lddy, dy_dtype, T, d}, x = {x_dev, ldx, x_dtype, T, d};
     for (const Rows *r : {&dx, &dy, &x})
         if (const char *bad = rows_wrong(*r)) return ops_fail(OMOE_ERR_INVALID, fn, bad);
-    if (rows_overlap(dx, dy) || rows_overlap(dx, x)) return ops_fail(OMOE_ERR_INVALID, fn, "an output overlaps another buffer");
     if (T > 0 && (!mean_dev || !rstd_dev)) return ops_fail(OMOE_ERR_INVALID, fn, "null buffer");
     if (misaligned(gamma_dev, 4) || misaligned(mean_dev, 4) || misaligned(rstd_dev, 4) || misaligned(dgamma_dev, 4) ||
         misaligned(dbeta_dev, 4))
         return ops_fail(OMOE_ERR_INVALID, fn, "fp32 buffers must be 4-byte aligned");
     if (workspace_bytes < omoe_layer_norm_backward_workspace(T, d) || !workspace_dev || misaligned(workspace_dev, 32))
         return ops_fail(OMOE_ERR_INVALID, fn, "the workspace is missing, misaligned or too small");
+    const Rows all[] = {dx, words(dgamma_dev, d), words(dbeta_dev, d), words(workspace_dev, omoe_layer_norm_backward_workspace(T, d) / 4),
+                        dy, x, words(gamma_dev, d), words(mean_dev, T), words(rstd_dev, T)};
+    if (int rc = ops_apart(all, 9, 4, fn)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");

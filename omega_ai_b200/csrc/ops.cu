@@ -64,6 +64,13 @@ bool rows_overlap(const Rows &a, const Rows &b) {
     return true;
 }
 
+int ops_apart(const Rows *all, int n, int n_out, const char *fn) {
+    for (int i = 0; i < n_out; i++)
+        for (int j = i + 1; j < n; j++)
+            if (rows_overlap(all[i], all[j])) return ops_fail(OMOE_ERR_INVALID, fn, "an output overlaps another buffer");
+    return OMOE_OK;
+}
+
 }  // namespace omoe
 
 extern "C" const char *omoe_ops_error(void) { return omoe::g_ops_err; }

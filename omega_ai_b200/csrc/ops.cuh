@@ -22,13 +22,17 @@ struct Rows {
     int64_t ld;
     int32_t dtype;
     int64_t rows;
-    int32_t d;
+    int64_t d;
     size_t elem() const { return dtype == OMOE_BF16 ? 2 : 4; }
 };
 // nullptr, or what is wrong with it.
 const char *rows_wrong(const Rows &r);
+// n contiguous elements of 4 bytes; none where p is null
+inline Rows words(const void *p, int64_t n) { return {p, n, OMOE_F32, p && n > 0 ? 1 : 0, n}; }
 // True where an element of `a` is also one of `b`.  Two column windows of the same matrix do not overlap.
 bool rows_overlap(const Rows &a, const Rows &b);
+// Status of a call whose first n_out buffers are written, with the text set: none of them may meet another one.
+int ops_apart(const Rows *all, int n, int n_out, const char *fn);
 // True when every group of 8 elements of a row is aligned to its size (16 bytes of bf16, 32 of fp32).
 inline bool rows_vector(const Rows &r) {
     return r.d % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % (8 * r.elem()) == 0 && (r.rows <= 1 || r.ld % 8 == 0);

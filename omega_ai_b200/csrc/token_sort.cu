@@ -416,14 +416,15 @@ int check_plan(const omoe_sort *p, const char *fn) {
     return OMOE_OK;
 }
 
-int check_rows(const Rows *const *m, int n, int n_out, const char *fn) {
+int check_rows(const Rows *m, int n, const char *fn) {
     for (int i = 0; i < n; i++)
-        if (const char *bad = rows_wrong(*m[i])) return ops_fail(OMOE_ERR_INVALID, fn, bad);
-    for (int i = 0; i < n_out; i++)  // outputs come first
-        for (int j = i + 1; j < n; j++)
-            if (rows_overlap(*m[i], *m[j])) return ops_fail(OMOE_ERR_INVALID, fn, "an output overlaps another buffer");
+        if (const char *bad = rows_wrong(m[i])) return ops_fail(OMOE_ERR_INVALID, fn, bad);
     return OMOE_OK;
 }
+// The plan's buffers as a call on rows reads them.
+Rows pos_of(const omoe_sort *p) { return words(p->pos, (int64_t)p->n_tokens * p->top_k); }
+Rows counts_of(const omoe_sort *p) { return words(p->counts, p->n_experts); }
+Rows offsets_of(const omoe_sort *p) { return words(p->offsets, (int64_t)p->n_experts + 1); }
 
 // The CTAs of the largest cluster that the current device can hold with all of kPlanSmem, asked once per device.
 cudaError_t plan_ctas(int *most) {
@@ -480,6 +481,9 @@ int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cud
     if (int rc = check_plan(plan, fn)) return rc;
     if (plan->n_tokens > 0 && !topk_idx_dev) return ops_fail(OMOE_ERR_INVALID, fn, "null buffer");
     if (misaligned(topk_idx_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "topk_idx_dev must be 4-byte aligned");
+    const Rows all[] = {pos_of(plan), words(plan->perm, plan->rows_cap), counts_of(plan), offsets_of(plan),
+                        words(topk_idx_dev, (int64_t)plan->n_tokens * plan->top_k)};
+    if (int rc = ops_apart(all, 5, 4, fn)) return rc;
     const int n = plan->n_tokens * plan->top_k, E = plan->n_experts;  // below 2^31: check_plan
     int most = 0;  // CTAs of a cluster
     if (cudaError_t e = plan_ctas(&most)) return ops_launched(e, fn);
@@ -517,8 +521,9 @@ int omoe_sort_rows(const omoe_sort *plan, const void *x_dev, int64_t ldx, int32_
     if (int rc = check_plan(plan, fn)) return rc;
     const int T = plan->n_tokens, E = plan->n_experts;
     const Rows x = {x_dev, ldx, x_dtype, T, d}, xs = {xs_dev, ldxs, xs_dtype, plan->rows_cap, d};
-    const Rows *all[] = {&xs, &x};
-    if (int rc = check_rows(all, 2, 1, fn)) return rc;
+    const Rows all[] = {xs, x, pos_of(plan), counts_of(plan), offsets_of(plan)};
+    if (int rc = check_rows(all, 2, fn)) return rc;
+    if (int rc = ops_apart(all, 5, 1, fn)) return rc;
     if (T == 0) return ops_ok();
     const bool vec = rows_vector(x) && rows_vector(xs);
     const int slices = pad_slices(plan->row_align), pads = E * slices;
@@ -542,9 +547,10 @@ static int unsort(const omoe_sort *plan, const void *ys_dev, int64_t ldys, int32
     if (int rc = check_plan(plan, fn)) return rc;
     const int T = plan->n_tokens;
     const Rows y = {y_dev, ldy, y_dtype, T, d}, ys = {ys_dev, ldys, ys_dtype, T ? plan->rows_cap : 0, d};
-    const Rows *all[] = {&y, &ys};
-    if (int rc = check_rows(all, 2, 1, fn)) return rc;
+    const Rows all[] = {y, ys, words(w_dev, (int64_t)T * plan->top_k), pos_of(plan)};
+    if (int rc = check_rows(all, 2, fn)) return rc;
     if (misaligned(w_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
+    if (int rc = ops_apart(all, 4, 1, fn)) return rc;
     if (T == 0) return ops_ok();
     const bool vec = rows_vector(y) && rows_vector(ys);
     return by_chunk(vec, T, d, true, [&](auto v, auto u) {
@@ -582,9 +588,11 @@ int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev, int64_t
     const int T = plan->n_tokens, E = plan->n_experts, k = plan->top_k;
     const Rows dys = {dys_dev, lddys, ys_dtype, T ? plan->rows_cap : 0, d}, dy = {dy_dev, lddy, dy_dtype, T, d};
     const Rows ys = {ys_dev, ldys, ys_dtype, T && dw_dev ? plan->rows_cap : 0, d};
-    const Rows *all[] = {&dys, &dy, &ys};
-    if (int rc = check_rows(all, dw_dev ? 3 : 2, 1, fn)) return rc;
+    const Rows rows[] = {dys, dy, ys};
+    if (int rc = check_rows(rows, dw_dev ? 3 : 2, fn)) return rc;
     if (misaligned(w_dev, 4) || misaligned(dw_dev, 4)) return ops_fail(OMOE_ERR_INVALID, fn, "the weights must be 4-byte aligned");
+    const Rows all[] = {dys, words(dw_dev, (int64_t)T * k), dy, ys, words(w_dev, (int64_t)T * k), pos_of(plan), counts_of(plan), offsets_of(plan)};
+    if (int rc = ops_apart(all, 8, 2, fn)) return rc;
     if (T == 0) return ops_ok();
     const int slices = pad_slices(plan->row_align);
     const bool vec = rows_vector(dys) && rows_vector(dy) && (!dw_dev || rows_vector(ys));

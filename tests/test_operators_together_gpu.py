@@ -90,3 +90,84 @@ def test_norm_in_front_of_the_layer_and_its_gradients_clipped():
     assert abs(float(after) / (0.01 * float(ref)) - 1) <= 1e-4
     assert all(((a == 0) == (b == 0)).all() for a, b in zip(grads, before))
     layer.close()
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from omega_ai_b200 import GradList, TokenSort, layer_norm, layer_norm_backward
+torch.manual_seed(0)
+x, g, b = torch.randn(300, 264, device="cuda"), torch.randn(264, device="cuda"), torch.randn(264, device="cuda")
+idx = torch.randint(0, 8, (300, 2), dtype=torch.int32, device="cuda")
+w, grads = torch.rand(300, 2, device="cuda"), [torch.randn(5000, device="cuda"), torch.randn(7, device="cuda")]
+sort = TokenSort(300, 2, 8, row_align=16)
+out = [torch.empty_like(t) for t in grads]
+clip = GradList(grads, out=out)
+def step():
+    h, mean, rstd = layer_norm(x, g, b, stats=True)
+    sort.plan(idx)
+    xs = sort.sort(h)
+    y = sort.unsort(xs, w)
+    dys, dw = sort.unsort_backward(y, xs, w)
+    dh = sort.sort_backward(dys)
+    return (y, dw, clip.clip(0.5), *layer_norm_backward(dh, x, g, mean, rstd))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got] + [t.clone() for t in out]
+want = list(step()) + out
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """Nothing has to be called once before a capture: attributes and occupancy are asked for while one is on."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "same" in p.stdout, p.stderr[-2000:]
+
+
+def test_eager_and_captured_calls_side_by_side():
+    """A captured step is replayed on one stream while the same operators run eagerly on another, on other data."""
+    from omega_ai_b200 import TokenSort, layer_norm, layer_norm_backward
+
+    def build(T, d, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x, dy = torch.randn(T, d, generator=g, device="cuda"), torch.randn(T, d, generator=g, device="cuda")
+        idx = torch.randint(0, 16, (T, 3), generator=g, dtype=torch.int32, device="cuda")
+        w, sort = torch.rand(T, 3, generator=g, device="cuda"), TokenSort(T, 3, 16)
+
+        def step():
+            h, mean, rstd = layer_norm(x, stats=True)
+            sort.plan(idx)
+            xs = sort.sort(h)
+            dys, dw = sort.unsort_backward(dy, xs, w)
+            return (sort.unsort(xs, w), dw, *layer_norm_backward(sort.sort_backward(dys), x, None, mean, rstd))
+
+        return step
+
+    one, two = build(3000, 1024, 1), build(1777, 520, 2)
+    want_one, want_two = [t.clone() for t in one()], [t.clone() for t in two()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got_one = one()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):
+        with torch.cuda.stream(a):
+            graph.replay()
+        with torch.cuda.stream(b):
+            got_two = two()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got_one, want_one))
+    assert all(torch.equal(x, y) for x, y in zip(got_two, want_two))
