@@ -18,12 +18,12 @@ constexpr int kPlanWarps = 32;
 constexpr int kPlanBatch = 8;    // picks a lane loads together
 constexpr int kPlanCtasMax = 16;  // the largest cluster; 8 where the device cannot hold one of 16
 constexpr size_t kPlanSmem = 220 * 1024;
-static_assert(sizeof(int32_t) * (OMOE_SORT_MAX_EXPERTS * (5 + kPlanWarps) + 1) <= kPlanSmem, "the tables of the most experts fit");
+static_assert(sizeof(int32_t) * (OMOE_SORT_MAX_EXPERTS * (4 + kPlanCtasMax + kPlanWarps) + 1) <= kPlanSmem, "the tables of the most experts fit");
 
 // One cluster does the whole plan.  Every warp owns a contiguous run of picks and counts its picks of every expert in
 // shared memory, numbering them as it goes: lanes with the same expert are found by ballots over the bits of its number (a warp-wide
-// match takes longer the more experts meet in a warp).  After sums over the warps and, through distributed shared memory,
-// over the CTAs every warp knows where its first pick of each expert goes.  A run of up to 256 picks stays in
+// match takes longer the more experts meet in a warp).  After sums over the warps, which every CTA stores into the shared memory of
+// all, and over the CTAs every warp knows where its first pick of each expert goes.  A run of up to 256 picks stays in
 // registers, a longer one keeps its numbers in pos meanwhile.
 // perm is a scatter: written pick by pick every store touches up to 32 lines, and eight SMs have to make them all (5 of 13 us for 49152
 // picks on 64 experts).  So the CTA's picks are put in order in shared memory first, `list` of them at most, and leave
@@ -35,8 +35,10 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     extern __shared__ int32_t sm[];
     cg::cluster_group cluster = cg::this_cluster();
     const int nw = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int32_t *s_total = sm;              // [E] this CTA's picks of every expert, read by the others
-    int32_t *s_count = s_total + E;     // [E] all picks
+    const int ctas = cluster.num_blocks(), cta = cluster.block_rank();
+    int32_t *s_totals = sm;             // [CTAs][E] the CTAs' picks of every expert, each stored by the CTA itself
+    int32_t *s_total = s_totals + cta * E;
+    int32_t *s_count = s_totals + ctas * E;  // [E] all picks
     int32_t *s_first = s_count + E;     // [E+1] first row of every expert
     int32_t *s_start = s_first + E + 1; // [E] first row of this CTA's picks of the expert
     int32_t *s_local = s_start + E;     // [E] where they start in the CTA's list
@@ -44,8 +46,9 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
     int32_t *s_list = s_hist + nw * E;  // [list] pick numbers by expert
     uint16_t *s_expert = reinterpret_cast<uint16_t *>(s_list + list);  // [list]
     int32_t *hist = s_hist + warp * E;
-    const int ctas = cluster.num_blocks(), cta = cluster.block_rank();
 
+    // the others' shared memory may be stored to once all CTAs have started; waited for below
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_trigger();
     for (int e = lane; e < E; e += 32) hist[e] = 0;
     const int64_t lo64 = (int64_t)(cta * nw + warp) * warp_run;
@@ -80,6 +83,7 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
         }
     }
     __syncthreads();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int run = 0;
 #pragma unroll 8
@@ -88,16 +92,15 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
             s_hist[w * E + e] = run;
             run += c;
         }
-        s_total[e] = run;
+        for (int c = 0; c < ctas; c++) cluster.map_shared_rank(s_total, c)[e] = run;
     }
-    if (ctas > 1) cluster.sync();
+    if (ctas > 1) cluster.sync();  // the last access to another CTA's memory
     else __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int before = 0, all = 0;
-#pragma unroll
-        for (int c = 0; c < kPlanCtasMax; c++) {
-            if (c >= ctas) break;
-            const int v = c == cta ? s_total[e] : cluster.map_shared_rank(s_total, c)[e];
+#pragma unroll 4
+        for (int c = 0; c < ctas; c++) {
+            const int v = s_totals[c * E + e];
             if (c < cta) before += v;
             all += v;
         }
@@ -170,7 +173,6 @@ sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int r
             if (row < rows_cap) perm[row] = s_list[q];
         }
     }
-    if (ctas > 1) cluster.sync();  // the others may still read this CTA's totals
 }
 
 // A warp takes one chunk of a token's columns: U vectors per lane.  Rows of up to 256 columns get one (a warp that has nothing to do for
@@ -493,7 +495,7 @@ int omoe_sort_plan(const omoe_sort *plan, const int32_t *topk_idx_dev, void *cud
     while (ctas < most && want > ctas * kPlanWarps) ctas *= 2;
     const int warps = want < 8 ? 8 : want > kPlanWarps ? kPlanWarps : (int)want;  // eight for the experts' sums alone
     const int64_t run = round_up(((int64_t)n + ctas * warps - 1) / (ctas * warps), 32);
-    const size_t tables = sizeof(int32_t) * ((size_t)E * (5 + warps) + 1);
+    const size_t tables = sizeof(int32_t) * ((size_t)E * (4 + ctas + warps) + 1);
     int64_t list = warps * run;  // picks of a CTA; beyond what fits they are scattered one by one
     if (tables + list * 6 > kPlanSmem) list = 0;
     const size_t smem = tables + list * 6;
