@@ -5,6 +5,7 @@
 // the call itself take about 4.  The entry points are not linked: init() gets their addresses from the library
 // that native.py has loaded, so that there is one copy of it in the process.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -122,10 +123,14 @@ T *vec(const OptTensor &t, int64_t n, const char *name, const c10::Device &devic
     return static_cast<T *>(vector(t, n, name, device, type));
 }
 
-Tensor matrix_or_new(const OptTensor &out, int64_t rows, int64_t d, at::ScalarType type, const c10::Device &device) {
-    return out ? *out : at::empty({rows, d}, at::TensorOptions().dtype(type).device(device));
+// An uninitialised tensor on the GPU, without the way through the dispatcher.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const c10::Device &device) {
+    return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
-Tensor floats(at::IntArrayRef sizes, const c10::Device &device) { return at::empty(sizes, at::TensorOptions().dtype(at::kFloat).device(device)); }
+Tensor matrix_or_new(const OptTensor &out, int64_t rows, int64_t d, at::ScalarType type, const c10::Device &device) {
+    return out ? *out : fresh({rows, d}, type, device);
+}
+Tensor floats(at::IntArrayRef sizes, const c10::Device &device) { return fresh(sizes, at::kFloat, device); }
 
 int64_t width(const Tensor &t, const char *name) {
     if (t.dim() != 2) bad(std::string(name) + ": expected a matrix, got " + text(t.sizes()));
@@ -246,7 +251,7 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor &dy, c
     if (o.dtype != in.dtype) bad("out: must have the type of x");
     const int64_t bytes = lib.layer_norm_backward_workspace(fits(T, "x"), fits(d, "x"));
     if (bytes < 0) bad("x: no columns");
-    const Tensor ws = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+    const Tensor ws = fresh({bytes}, at::kByte, dev);
     OptTensor dgamma, dbeta;
     if (param_grads) {
         dgamma = floats({d}, dev);
@@ -283,7 +288,7 @@ struct GradList {
         list(out, to);
     }
     const omoe_tensor *target() const { return in_place ? nullptr : to.data(); }
-    Tensor workspace() const { return at::empty({OMOE_GRAD_WORKSPACE_BYTES}, at::TensorOptions().dtype(at::kByte).device(device)); }
+    Tensor workspace() const { return fresh({OMOE_GRAD_WORKSPACE_BYTES}, at::kByte, device); }
 
     Tensor norm() const {
         const On on(device);
