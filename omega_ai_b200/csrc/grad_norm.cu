@@ -302,7 +302,7 @@ cudaError_t tables(const omoe_tensor *grads, const omoe_tensor *out, int n, int 
             if (grads[i].count == 0) continue;
             const int elems = chunk_elems(grads[i].dtype);
             const int64_t c = (grads[i].count + elems - 1) / elems;
-            if (chunks + c > INT32_MAX) break;  // never for the first: count <= 2^42
+            if (chunks + c > INT32_MAX / 2) break;  // chunk numbers and a grid beyond them fit; never for the first: count <= 2^42
             t.e[t.n++] = {grads[i].ptr, out ? out[i].ptr : grads[i].ptr, grads[i].count, (int32_t)chunks, grads[i].dtype};
             chunks += c;
         }

@@ -25,8 +25,8 @@ static_assert(sizeof(int32_t) * (OMOE_SORT_MAX_EXPERTS * (4 + kPlanCtasMax + kPl
 // match takes longer the more experts meet in a warp).  After sums over the warps, which every CTA stores into the shared memory of
 // all, and over the CTAs every warp knows where its first pick of each expert goes.  A run of up to 256 picks stays in
 // registers, a longer one keeps its numbers in pos meanwhile.
-// perm is a scatter: written pick by pick every store touches up to 32 lines, and eight SMs have to make them all (5 of 13 us for 49152
-// picks on 64 experts).  So the CTA's picks are put in order in shared memory first, `list` of them at most, and leave
+// perm is a scatter: written pick by pick every store touches up to 32 lines, and few SMs have to make them all (by eight, 49152 picks on 64
+// experts took 13.5 us, through lists 10.8; sixteen CTAs that send their totals take 7.8).  So the CTA's picks are put in order in shared memory first, `list` of them at most, and leave
 // as one run per expert.  Bound by latency: the walk, the barriers, the copies.
 __global__ void __launch_bounds__(kPlanWarps * 32)
 sort_plan_kernel(const int32_t *__restrict__ idx, int n, int E, int align, int rows_cap, int warp_run, int list,
@@ -402,7 +402,7 @@ unsort_bwd_kernel(const DT *__restrict__ dy, int64_t lddy, const YT *__restrict_
 const char *plan_wrong(const omoe_sort *p) {
     if (!p) return "null plan";
     if (p->n_tokens < 0 || p->top_k < 1 || p->n_experts < 1 || p->row_align < 1) return "bad sizes in the plan";
-    if (!p->counts || !p->offsets || (p->n_tokens > 0 && (!p->pos || !p->perm))) return "null buffer in the plan";
+    if (!p->counts || !p->offsets || (p->n_tokens > 0 && !p->pos) || (p->rows_cap > 0 && !p->perm)) return "null buffer in the plan";
     if (misaligned(p->pos, 4) || misaligned(p->perm, 4) || misaligned(p->counts, 4) || misaligned(p->offsets, 4))
         return "the plan's buffers must be 4-byte aligned";
     return nullptr;

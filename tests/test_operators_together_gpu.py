@@ -171,3 +171,42 @@ def test_eager_and_captured_calls_side_by_side():
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got_one, want_one))
     assert all(torch.equal(x, y) for x, y in zip(got_two, want_two))
+
+
+def test_captured_across_streams_that_part_and_join():
+    """A capture that forks to a second stream and joins it again: the operators' launches depend on kernels, copies and events."""
+    from omega_ai_b200 import GradList, TokenSort, layer_norm
+
+    T, d = 500, 512
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, source = torch.zeros(T, d, device="cuda"), torch.randn(T, d, generator=g, device="cuda")
+    idx = torch.randint(0, 8, (T, 2), generator=g, dtype=torch.int32, device="cuda")
+    sort, grads = TokenSort(T, 2, 8, row_align=8), [torch.randn(30000, generator=g, device="cuda")]
+    clipped = [torch.zeros_like(grads[0])]
+    clip = GradList(grads, out=clipped)
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        x.copy_(source)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            sort.plan(idx)
+            norm = clip.clip(0.5)
+        h = layer_norm(x)
+        main.wait_stream(side)
+        xs = sort.sort(h, out=torch.zeros(sort.rows_cap, d, device="cuda"))
+        return h, sort.unsort(xs), norm
+
+    want = [t.clone() for t in step()] + [clipped[0].clone()]
+    torch.cuda.synchronize()
+    clipped[0].zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        x.zero_()
+        sort.pos.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip([*got, clipped[0]], want))

@@ -55,6 +55,8 @@ def test_sort_refusals(native):
     L, p = native.lib(), C.byref(plan(native))
     refused(native, L.omoe_sort_plan(None, P, None), INVALID, "null plan")
     refused(native, L.omoe_sort_plan(p, None, None), INVALID, "null")
+    # no tokens, but rows that the plan marks as empty
+    refused(native, L.omoe_sort_plan(C.byref(plan(native, T=0, cap=64, pos=None, perm=None)), None, None), INVALID, "null")
     refused(native, L.omoe_sort_plan(p, P + 1, None), INVALID, "aligned")
     for idx in (P, P + 28, 2 * P, 3 * P + 28, 4 * P + 32):  # the picks in a buffer of the plan
         refused(native, L.omoe_sort_plan(p, idx, None), INVALID, "overlaps")

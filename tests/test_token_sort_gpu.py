@@ -85,6 +85,24 @@ def test_plan_of_no_tokens():
     assert sort.unsort(torch.empty(0, 16, device="cuda")).shape == (0, 16)
 
 
+def test_more_rows_than_needed_and_none_at_all():
+    """rows_cap may be larger than it has to be: the plan marks the rows behind the last expert's, with no tokens too."""
+    import ctypes as C
+
+    from omega_ai_b200 import native
+
+    L = native.lib()
+    for T in (0, 3):
+        new = lambda n: torch.full((n,), -77, dtype=torch.int32, device="cuda")
+        pos, perm, counts, offsets = new(max(1, 2 * T)), new(1000), new(8), new(9)
+        idx = torch.tensor([[1, 7], [0, 9], [7, 1]], dtype=torch.int32, device="cuda")
+        p = native.Sort(T, 2, 8, 4, 1000, pos.data_ptr(), perm.data_ptr(), counts.data_ptr(), offsets.data_ptr())
+        assert L.omoe_sort_plan(C.byref(p), idx.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        want = plain_plan(idx[:T].cpu().numpy().reshape(T, 2), 8, 4, 1000)
+        for got, ref in zip((pos[:2 * T].reshape(T, 2), perm, counts, offsets), want):
+            np.testing.assert_array_equal(got.cpu().numpy(), ref)
+
+
 def matrix(rows, d, dtype, layout, seed):
     """[rows, d] of N(0, 1) in one of several layouts, and the whole buffer it lies in."""
     g = torch.Generator(device="cuda").manual_seed(seed)
