@@ -130,6 +130,15 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const c10::Device &devi
 Tensor matrix_or_new(const OptTensor &out, int64_t rows, int64_t d, at::ScalarType type, const c10::Device &device) {
     return out ? *out : fresh({rows, d}, type, device);
 }
+// A vector of n floats and a second one behind it in the same storage: what lives and dies together takes one allocation.
+std::pair<Tensor, Tensor> two_floats(int64_t n, const c10::Device &device) {
+    Tensor a = fresh({2 * n}, at::kFloat, device);
+    auto b = c10::make_intrusive<c10::TensorImpl>(c10::Storage(a.storage()), a.key_set(), a.dtype());
+    b->set_sizes_contiguous({n});
+    b->set_storage_offset(n);
+    a.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return {a, Tensor(std::move(b))};
+}
 Tensor floats(at::IntArrayRef sizes, const c10::Device &device) { return fresh(sizes, at::kFloat, device); }
 
 int64_t width(const Tensor &t, const char *name) {
@@ -229,10 +238,7 @@ py::object layer_norm(const Tensor &x, const OptTensor &gamma, const OptTensor &
     const On on(dev);
     Tensor y = matrix_or_new(out, T, d, dtype.value_or(x.scalar_type()), dev), mean, rstd;
     const Matrix o(y, T, d, "out", dev);
-    if (stats) {
-        mean = floats({T}, dev);
-        rstd = floats({T}, dev);
-    }
+    if (stats) std::tie(mean, rstd) = two_floats(T, dev);
     check(lib.layer_norm(in.p, in.ld, in.dtype, g, b, (float)eps, o.p, o.ld, o.dtype, stats ? static_cast<float *>(mean.data_ptr()) : nullptr,
                          stats ? static_cast<float *>(rstd.data_ptr()) : nullptr, fits(T, "x"), fits(d, "x"), on.stream));
     if (!stats) return py::cast(y);
@@ -253,10 +259,7 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor &dy, c
     if (bytes < 0) bad("x: no columns");
     const Tensor ws = fresh({bytes}, at::kByte, dev);
     OptTensor dgamma, dbeta;
-    if (param_grads) {
-        dgamma = floats({d}, dev);
-        dbeta = floats({d}, dev);
-    }
+    if (param_grads) std::tie(dgamma, dbeta) = two_floats(d, dev);
     check(lib.layer_norm_backward(g.p, g.ld, g.dtype, in.p, in.ld, in.dtype, gm, m, r, o.p, o.ld,
                                   dgamma ? static_cast<float *>(dgamma->data_ptr()) : nullptr, dbeta ? static_cast<float *>(dbeta->data_ptr()) : nullptr,
                                   (int32_t)T, (int32_t)d, ws.data_ptr(), bytes, on.stream));
