@@ -364,7 +364,7 @@ OMOE_API const char *omoe_ops_error(void);
  * same expert may be picked twice by a token.  rows_cap must be at least omoe_sort_rows_cap(...), which returns
  * T*top_k plus the padding that the experts with picks can need, or a negative status.
  * Limits: n_experts <= OMOE_SORT_MAX_EXPERTS, top_k <= 16, rows_cap <= 0x7fff0000; leading dimensions
- * of all the operators: at most 2^30.
+ * of all the operators: below 2^30.
  *
  * With N picks that have a row:
  *   omoe_sort_rows            xs[pos[t,j], :] = x[t, :] for every pick; padding rows (inside [0, offsets[E])) are

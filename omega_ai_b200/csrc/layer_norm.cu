@@ -270,13 +270,14 @@ struct Ahead {
                 }
         __syncwarp();
     }
-    __device__ __forceinline__ void fetch(int stage, const T *row, int d) const {
+    // from: the row's element `col`
+    __device__ __forceinline__ void fetch(int stage, const T *from, int d) const {
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int q = 0; q < kPieces; q++) {
-                const int c = col + p * G * 8 + q * 128;
-                if (c < d) copy16(put + stage * kStage + p * kVector + q * 512, row + c);
+                const int c = p * G * 8 + q * 128;
+                if (col + c < d) copy16(put + stage * kStage + p * kVector + q * 512, from + c);
             }
     }
     // pairs 4p .. 4p + 3 of this thread
@@ -299,14 +300,15 @@ template <typename T, int B, int G, int P, int S>
 struct Ahead<T, B, 1, G, P, S> {
     static constexpr int kStage = 0;
     Frag<T, 1> next[P];
-    __device__ __forceinline__ Ahead(uint32_t, int) {
+    int col;
+    __device__ __forceinline__ Ahead(uint32_t, int) : col(threadIdx.x % G) {
 #pragma unroll
         for (int p = 0; p < P; p++) next[p].zero();
     }
-    __device__ __forceinline__ void fetch(int, const T *row, int d) {
+    __device__ __forceinline__ void fetch(int, const T *from, int d) {
 #pragma unroll
         for (int p = 0; p < P; p++)
-            if (p * G + (int)(threadIdx.x % G) < d) next[p].load(row + p * G + threadIdx.x % G);
+            if (col + p * G < d) next[p].load(from + p * G);
     }
     // all of this thread's elements, two by two
     __device__ __forceinline__ void take(int, int p, f2 (&v)[P / 2]) const {
@@ -357,6 +359,7 @@ struct Part {
             }
         }
     }
+    // p: element col(0) of the row
     template <typename T>
     __device__ __forceinline__ void store(T *p, int q, const f2 (&v)[kPairs]) const {
         float w[2 * kPairs];
@@ -366,14 +369,20 @@ struct Part {
             if (!has(q)) return;
             Frag<T, 8> f;
             f.set(w);
-            f.store(p + col(q));
+            f.store(p + q * G * 8);
         } else {
 #pragma unroll
             for (int i = 0; i < 2 * kPairs; i++)
-                if (in_row() + i * G < d) p[in_row() + i * G] = (T)w[i];
+                if (in_row() + i * G < d) p[i * G] = (T)w[i];
         }
     }
 };
+
+// p, rows of `bytes` bytes further on.
+template <typename T>
+__device__ __forceinline__ T *rows_on(T *p, int rows, uint32_t bytes) {
+    return reinterpret_cast<T *>(reinterpret_cast<uintptr_t>(p) + (uint64_t)(uint32_t)rows * bytes);
+}
 
 // Blocks that share an SM: what the registers allow.
 template <int G>
@@ -384,8 +393,9 @@ constexpr int kBwdBlocks = P > 4 || (V == 8 && P > 1) ? 1 : 1024 / kBwdBlock<XT,
 // shuffles and the loads of gamma and beta; fp32 and narrower rows are faster one by one.
 template <typename XT, int V, int G>
 constexpr int kFwdRows = V == 8 && G >= 512 && sizeof(XT) == 2 ? 2 : 1;
-// Stages that fit a block's share of shared memory: four, six where two long rows are at work (16384 x 4096 of bf16 forward 47.7 us
-// with four and 51.0 with six, 4096 x 16384 66.7 and 58.2).
+// Stages that fit a block's share of shared memory: four; six where two long rows are at work (16384 x 4096 of bf16 forward 47.7 us with four
+// and 51.0 with six, 4096 x 16384 66.7 and 58.2); two where two backward blocks of long fp32 rows share an SM (x 4096 to bf16, 8192 to
+// 30011 rows: 52 to 186 us, with four 57 to 215).
 constexpr int stages(int stage_bytes, int blocks, int most) {
     const int fit = stage_bytes ? 212992 / blocks / stage_bytes : 2;
     return fit > most ? most : fit;
@@ -393,7 +403,8 @@ constexpr int stages(int stage_bytes, int blocks, int most) {
 template <typename XT, int V, int G, int P>
 constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, P > 1 ? 2 + 2 * kFwdRows<XT, V, G> : 4);
 template <typename XT, typename YT, int V, int G, int P>
-constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>, 4);
+constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>,
+                                                  G == 512 && sizeof(XT) == 4 ? 2 : 4);
 
 template <int B, int G>
 __device__ __forceinline__ void row_barrier() {
@@ -464,8 +475,8 @@ struct Param {
 
 template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kFwdBlock<G>, kFwdBlocks<G>)
-norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
-            YT *__restrict__ y, int ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
+norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
+            YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
     using Mine = Part<V, G, P>;
     constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G>, Q = Mine::kGroups, N = Mine::kPairs;
     static_assert(S >= 2 * R, "rows are read from some stages while others fill");
@@ -480,28 +491,27 @@ norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, 
     pdl_wait();
     const Param<V, G, P> scale(gamma, part, 1.f), shift(beta, part, 0.f);
     int t = blockIdx.x * (B / G) + group;  // T and the rows of 2 S strides stay below 2^31: kRowsMax
-    int next = t, fill = 0;                        // the row to fetch and its stage
-    auto fetch = [&]() {
-        if (next < T) ahead.fetch(fill, x + (int64_t)next * ldx, d);
+    int next = t;  // the row to fetch
+    x += ahead.col;
+    y += part.col(0);
+    auto fetch = [&](int stage) {
+        if (next < T) ahead.fetch(stage, rows_on(x, next, x_pitch), d);
         copies_commit();
         next += step;
-        fill = fill + 1 == S ? 0 : fill + 1;
     };
 #pragma unroll
-    for (int i = 0; i < S - R; i++) fetch();
+    for (int i = 0; i < S - R; i++) fetch(i);
     float *s_mean = s_sum[0] + group * (2 * G / 32), *s_var = s_sum[1] + group * (2 * G / 32);
-    for (int stage = 0; t < T; t += R * step) {
+    auto rows = [&](int stage) {  // R rows from `stage` on
         f2 v[R][Q][N];
         float sum[2] = {0.f, 0.f}, mean[2], rstd[2];
         copies_wait<S - 2 * R>();
 #pragma unroll
-        for (int r = 0; r < R; r++) {
+        for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int q = 0; q < Q; q++) ahead.take(stage, q, v[r][q]);
-            stage = stage + 1 == S ? 0 : stage + 1;
-        }
+            for (int q = 0; q < Q; q++) ahead.take(stage + r, q, v[r][q]);
 #pragma unroll
-        for (int r = 0; r < R; r++) fetch();
+        for (int r = 0; r < R; r++) fetch((stage + S - R + r) % S);
 #pragma unroll
         for (int r = 0; r < R; r++) {
             f2 pair = 0ull;
@@ -553,8 +563,19 @@ norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, 
                 f2 out[N];
 #pragma unroll
                 for (int i = 0; i < N; i++) out[i] = fma2(mul2(v[r][q][i], rr), w[i], b[i]);
-                part.store(y + (int64_t)(t + r * step) * ldy, q, out);
+                part.store(rows_on(y, t + r * step, y_pitch), q, out);
             }
+        }
+    };
+    // a copy of the loop's body for every stage that a row can lie in, so that stages are constants
+    constexpr int kPhases = V == 1 ? 1 : S / R;
+    static_assert(V == 1 || S % R == 0, "whole groups of rows");
+    while (t < T) {
+#pragma unroll
+        for (int phase = 0; phase < kPhases; phase++) {
+            if (t >= T) break;
+            rows(phase * R);
+            t += R * step;
         }
     }
 }
@@ -563,8 +584,8 @@ norm_kernel(const XT *__restrict__ x, int ldx, const float *__restrict__ gamma, 
 // several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
 template <typename XT, typename YT, int V, int G, int P>
 __global__ void __launch_bounds__(kBwdBlock<XT, V, G, P>, kBwdBlocks<XT, V, G, P>)
-norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, int ldx, const float *__restrict__ gamma,
-                const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, int lddx,
+norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma,
+                const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, uint32_t dx_pitch,
                 float *__restrict__ partial, int T, int d) {
     using Mine = Part<V, G, P>;
     constexpr int B = kBwdBlock<XT, V, G, P>, S = kBwdStages<XT, YT, V, G, P>, Q = Mine::kGroups, N = Mine::kPairs;
@@ -588,10 +609,13 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
     pdl_wait();
     const Param<V, G, P> scale(gamma, part, 1.f);
     int t = blockIdx.x * (B / G) + group, next = t;
+    x += ahead_x.col;
+    dy += ahead_y.col;
+    dx += part.col(0);
     auto fetch = [&](int stage) {
         if (next < T) {
-            ahead_x.fetch(stage, x + (int64_t)next * ldx, d);
-            ahead_y.fetch(stage, dy + (int64_t)next * lddy, d);
+            ahead_x.fetch(stage, rows_on(x, next, x_pitch), d);
+            ahead_y.fetch(stage, rows_on(dy, next, dy_pitch), d);
         }
         copies_commit();
         next += step;
@@ -603,10 +627,9 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
         m = mean[t];
         r = rstd[t];
     }
-    for (int stage = 0, odd = 0; t < T; t += step, odd ^= 1) {
+    auto row = [&](int stage, int odd) {
         f2 h[Q][N], g[Q][N], sum_g = 0ull, sum_gh = 0ull;
         const f2 minus = pack2(-m, -m), rr = pack2(r, r);
-        const int refill = stage == 0 ? S - 1 : stage - 1;
         if (t + step < T) {
             m = mean[t + step];
             r = rstd[t + step];
@@ -616,7 +639,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
             ahead_x.take(stage, 0, h[0]);
             ahead_y.take(stage, 0, g[0]);
         }
-        fetch(refill);
+        fetch((stage + S - 1) % S);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             if constexpr (kAgain) {
@@ -654,9 +677,18 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
             }
 #pragma unroll
             for (int i = 0; i < N; i++) out[i] = mul2(fma2(h[q][i], slope, add2(g[q][i], less)), rr);
-            part.store(dx + (int64_t)t * lddx, q, out);
+            part.store(rows_on(dx, t, dx_pitch), q, out);
         }
-        stage = stage + 1 == S ? 0 : stage + 1;
+    };
+    // as in the forward kernel; an even number of copies, for the two sets of sums that take turns
+    constexpr int kPhases = S % 2 ? 2 * S : S;
+    while (t < T) {
+#pragma unroll
+        for (int phase = 0; phase < kPhases; phase++) {
+            if (t >= T) break;
+            row(phase % S, phase % 2);
+            t += step;
+        }
     }
     if (!partial) return;
     // column sums of the block: the rows' groups joined through shared memory, in order
@@ -664,8 +696,8 @@ norm_bwd_kernel(const YT *__restrict__ dy, int lddy, const XT *__restrict__ x, i
     if constexpr (G == B) {
 #pragma unroll
         for (int q = 0; q < Q; q++) {
-            part.store(sums, q, dg[q]);
-            part.store(sums + d, q, db[q]);
+            part.store(sums + part.col(0), q, dg[q]);
+            part.store(sums + d + part.col(0), q, db[q]);
         }
     } else {
         constexpr int W = G * P * V;  // columns a group covers
@@ -802,7 +834,8 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
                          if (e != cudaSuccess) return;
                          const int blocks = ceil_div(T, kFwdBlock<G> / G), most = kFwdBlocks<G> * sms;
                          e = launch_ex(norm_kernel<XT, YT, V, G, P>, dim3(blocks < most ? blocks : most), dim3(kFwdBlock<G>), smem, s, ops_pdl(),
-                                       static_cast<const XT *>(x_dev), (int)ldx, gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev), (int)ldy,
+                                       static_cast<const XT *>(x_dev), (uint32_t)(ldx * sizeof(XT)), gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev),
+                                       (uint32_t)(ldy * sizeof(YT)),
                                        mean_dev, rstd_dev, T, d);
                      }))
             return e;
@@ -867,8 +900,9 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
                                       int most = kBwdBlocks<XT, V, G, P> * sms;
                                       most = most < kBwdBlocksMax ? most : kBwdBlocksMax;
                                       sums = blocks < most ? blocks : most;
-                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(B), smem, s, ops_pdl(), g, (int)lddy, in,
-                                                    (int)ldx, gamma_dev, mean_dev, rstd_dev, static_cast<XT *>(dx_dev), (int)lddx,
+                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(B), smem, s, ops_pdl(), g,
+                                                    (uint32_t)(lddy * sizeof(YT)), in, (uint32_t)(ldx * sizeof(XT)), gamma_dev, mean_dev,
+                                                    rstd_dev, static_cast<XT *>(dx_dev), (uint32_t)(lddx * sizeof(XT)),
                                                     params ? partial : nullptr, T, d);
                                   }
                               }) && (e != cudaSuccess || sums > 0)) {

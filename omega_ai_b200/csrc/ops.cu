@@ -41,7 +41,7 @@ bool ops_pdl() {
 const char *rows_wrong(const Rows &r) {
     if (r.dtype != OMOE_F32 && r.dtype != OMOE_BF16) return "a dtype is neither OMOE_F32 nor OMOE_BF16";
     if (r.d <= 0) return "d must be positive";
-    if (r.ld < r.d || r.ld > ((int64_t)1 << 30)) return "a leading dimension is smaller than d or out of range";
+    if (r.ld < r.d || r.ld >= ((int64_t)1 << 30)) return "a leading dimension is smaller than d or out of range";
     if (r.rows > 0 && !r.p) return "null buffer";
     if (misaligned(r.p, r.elem())) return "a buffer is not aligned to its element type";
     return nullptr;
