@@ -390,21 +390,22 @@ constexpr int kFwdBlocks = 1024 / kFwdBlock<G>;
 template <typename XT, int V, int G, int P>
 constexpr int kBwdBlocks = P > 4 || (V == 8 && P > 1) ? 1 : 1024 / kBwdBlock<XT, V, G, P>;
 // Rows that a forward block's threads take at a time.  Where many threads share a row of bf16, two rows share their barriers and
-// shuffles and the loads of gamma and beta; fp32 and narrower rows are faster one by one.
+// shuffles (16384 x 4096: 44 us, one by one 50; 40000 x 1536: 44 and 55); fp32 is bound by HBM either way, and narrower rows are
+// faster one by one (65536 x 1024: 49 us and 45).
 template <typename XT, int V, int G>
-constexpr int kFwdRows = V == 8 && G >= 512 && sizeof(XT) == 2 ? 2 : 1;
-// Stages that fit a block's share of shared memory: four; six where two long rows are at work (16384 x 4096 of bf16 forward 47.7 us with four
-// and 51.0 with six, 4096 x 16384 66.7 and 58.2); two where two backward blocks of long fp32 rows share an SM (x 4096 to bf16, 8192 to
-// 30011 rows: 52 to 186 us, with four 57 to 215).
+constexpr int kFwdRows = V == 8 && G >= 256 && sizeof(XT) == 2 ? 2 : 1;
+// Stages that fit a block's share of shared memory.  Forward two beside those of two goes (16384 x 4096 of bf16 with four 45.3 us, with six
+// 43.9).  Backward three for bf16 (with four 65536 x 256 takes 23.3 us, 22.4 with three), four for fp32, and two where two blocks
+// of long fp32 rows share an SM (x 4096 to bf16, 8192 to 30011 rows: 52 to 186 us, with four 57 to 215).
 constexpr int stages(int stage_bytes, int blocks, int most) {
     const int fit = stage_bytes ? 212992 / blocks / stage_bytes : 2;
     return fit > most ? most : fit;
 }
 template <typename XT, int V, int G, int P>
-constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, P > 1 ? 2 + 2 * kFwdRows<XT, V, G> : 4);
+constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, 2 + 2 * kFwdRows<XT, V, G>);
 template <typename XT, typename YT, int V, int G, int P>
 constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>,
-                                                  G == 512 && sizeof(XT) == 4 ? 2 : 4);
+                                                  sizeof(XT) == 2 ? 3 : G == 512 ? 2 : 4);
 
 template <int B, int G>
 __device__ __forceinline__ void row_barrier() {
