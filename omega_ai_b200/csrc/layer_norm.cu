@@ -131,52 +131,53 @@ norm_bwd_wide_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restri
     }
 }
 
-// Column sums of a slice of the rows: partial[slice][0][d] of dy * h, [1][d] of dy.  A warp takes every eighth row of 32 V columns.
+// Column sums of a slice of the rows: partial[slice][0][d] of dy * h, [1][d] of dy.  A thread has V columns of all of the slice's rows.
+constexpr int kColThreads = 256;
 template <typename XT, typename YT, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kColThreads)
 norm_cols_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__ x, int64_t ldx,
                  const float *__restrict__ mean, const float *__restrict__ rstd, float *__restrict__ partial, int T, int d,
                  int slice) {
-    __shared__ float s[2][8][32 * V + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * 32 * V, c = c0 + lane * V;
+    constexpr int U = V == 8 ? 2 : 4;  // rows whose loads are on their way together (twice as many take the registers of half the blocks)
+    const int64_t c = ((int64_t)blockIdx.x * kColThreads + threadIdx.x) * V;
     pdl_trigger();
     pdl_wait();
+    if (c >= d) return;
     const int64_t t0 = (int64_t)blockIdx.y * slice, t1 = min((int64_t)T, t0 + slice);
     float a[V], b[V];
 #pragma unroll
     for (int i = 0; i < V; i++) a[i] = b[i] = 0.f;
-    if (c < d) {
-#pragma unroll 4
-        for (int64_t t = t0 + warp; t < t1; t += 8) {
-            Frag<YT, V> fy;
-            Frag<XT, V> fx;
-            float g[V], h[V];
-            fy.load(dy + t * lddy + c);
-            fx.load(x + t * ldx + c);
-            fy.get(g);
-            fx.get(h);
-            const float m = mean[t], r = rstd[t];
+    for (int64_t t = t0; t < t1; t += U) {
+        Frag<YT, V> fy[U];
+        Frag<XT, V> fx[U];
+        float m[U], r[U];
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                a[i] = fmaf(g[i], (h[i] - m) * r, a[i]);
-                b[i] += g[i];
+        for (int u = 0; u < U; u++)
+            if (t + u < t1) {
+                fy[u].load(dy + (t + u) * lddy + c);
+                fx[u].load(x + (t + u) * ldx + c);
+                m[u] = mean[t + u];
+                r[u] = rstd[t + u];
             }
-        }
-    }
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        s[0][warp][lane * V + i] = a[i];
-        s[1][warp][lane * V + i] = b[i];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * V; i += 256) {
-        const int which = i / (32 * V), col = i % (32 * V);
-        if (c0 + col >= d) continue;
-        float sum = 0.f;
+        for (int u = 0; u < U; u++)
+            if (t + u < t1) {
+                float g[V], h[V];
+                fy[u].get(g);
+                fx[u].get(h);
 #pragma unroll
-        for (int w = 0; w < 8; w++) sum += s[which][w][col];
-        partial[((int64_t)blockIdx.y * 2 + which) * d + c0 + col] = sum;
+                for (int i = 0; i < V; i++) {
+                    a[i] = fmaf(g[i], (h[i] - m[u]) * r[u], a[i]);
+                    b[i] += g[i];
+                }
+            }
     }
+    float *to = partial + (int64_t)blockIdx.y * 2 * d + c;
+    Frag<float, V> f;
+    f.set(a);
+    f.store(to);
+    f.set(b);
+    f.store(to + d);
 }
 
 // ---- rows that fit a block's registers ----------------------------------------------------------------------------
@@ -748,12 +749,18 @@ norm_join_kernel(const float *__restrict__ partial, int n, int d, float *__restr
     if (lane == 0 && blockIdx.x * 32 + warp < d) out[blockIdx.x * 32 + warp] = sum;
 }
 
-// Row slices of the wide kernels whose column sums are kept apart.
-constexpr int kSlicesMax = 64;
+// Row slices of norm_cols_kernel, whose column sums are kept apart: as many as give every SM kColBlocks blocks, but eight at least, so that
+// no sum is longer than an eighth of the rows.
+constexpr int kSlicesMin = 8, kSlicesMax = 64, kColBlocks = 4;
 // Blocks of norm_bwd_kernel, and with that column sums kept apart: two on each of up to 160 SMs.
 constexpr int kBwdBlocksMax = 320;
 
-int slices_of(int T) { return T < kSlicesMax ? (T < 1 ? 1 : T) : kSlicesMax; }
+int slices_of(int T, int d, int per_thread, int sms) {
+    int want = ceil_div(sms * kColBlocks, ceil_div(d, kColThreads * per_thread));
+    want = want < kSlicesMin ? kSlicesMin : want;
+    const int most = T < kSlicesMax ? (T < 1 ? 1 : T) : kSlicesMax;
+    return want < most ? want : most;
+}
 
 // Calls f with the vector width, threads per row and vectors per thread (integral constants) for rows of width d, or
 // returns false where they do not fit a block's registers.  Vectors: the fewest threads that hold the row with one each, then two.
@@ -876,7 +883,7 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
     float *partial = static_cast<float *>(workspace_dev);
-    const int slices = slices_of(T), cols = ceil_div(d, 32);
+    const int cols = ceil_div(d, 32);
     const bool params = dgamma_dev || dbeta_dev;
     return ops_launched(by_types(x_dtype, dy_dtype, [&](auto *xt, auto *yt) {
         using XT = std::remove_pointer_t<decltype(xt)>;
@@ -910,13 +917,15 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
             if (e != cudaSuccess || !params) return e;
             return launch_ex(norm_join_kernel, dim3(cols, 2), dim3(1024), 0, s, ops_pdl(), partial, sums, d, dgamma_dev, dbeta_dev);
         }
+        int slices = 0;
         auto wide = [&](auto kern, auto cols_kern, int V) {
             cudaError_t e = cudaSuccess;
+            slices = slices_of(T, d, V, sms);
             if (T > 0)
                 e = launch_ex(kern, dim3(T), dim3(kWideThreads), 0, s, ops_pdl(), g, lddy, in, ldx, gamma_dev, mean_dev, rstd_dev,
                               static_cast<XT *>(dx_dev), lddx, d);
             if (e != cudaSuccess || !params) return e;
-            return launch_ex(cols_kern, dim3(ceil_div(d, 32 * V), slices), dim3(256), 0, s, ops_pdl(), g, lddy, in, ldx, mean_dev, rstd_dev,
+            return launch_ex(cols_kern, dim3(ceil_div(d, kColThreads * V), slices), dim3(kColThreads), 0, s, ops_pdl(), g, lddy, in, ldx, mean_dev, rstd_dev,
                              partial, T, d, ceil_div(T, slices));
         };
         e = vec ? wide(norm_bwd_wide_kernel<XT, YT, 8>, norm_cols_kernel<XT, YT, 8>, 8)

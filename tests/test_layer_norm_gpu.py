@@ -64,6 +64,8 @@ CASES = [
     (2, 16392, BF, BF, "aligned", "both", 1.0, 0.0),
     (2, 40000, BF, F32, "packed", "both", 1.0, 0.0),
     (1, 70001, F32, BF, "packed", "none", 1.0, 0.0),
+    (300, 20000, BF, BF, "packed", "both", 1.0, 0.0),
+    (150, 9001, F32, BF, "packed", "both", 1.0, 0.0),
     (70, 201, BF, F32, "odd", "both", 1.0, 0.0),
     (301, 401, BF, BF, "packed", "both", 1.0, 0.0),
     (9, 2047, F32, F32, "packed", "both", 1.0, 0.0),
