@@ -44,7 +44,7 @@ norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict_
     float v[V], sum = 0.f;
 #pragma unroll 4
     for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
-        f.load(row + c);
+        f.load_cached(row + c);
         f.get(v);
 #pragma unroll
         for (int i = 0; i < V; i++) sum += v[i];
@@ -53,7 +53,7 @@ norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict_
     sum = 0.f;
 #pragma unroll 4
     for (int c = threadIdx.x * V; c < d; c += kWideThreads * V) {
-        f.load(row + c);
+        f.load_cached(row + c);
         f.get(v);
 #pragma unroll
         for (int i = 0; i < V; i++) sum = fmaf(v[i] - mean, v[i] - mean, sum);
@@ -67,7 +67,7 @@ norm_wide_kernel(const XT *__restrict__ x, int64_t ldx, const float *__restrict_
         Frag<float, V> p;
         Frag<YT, V> out;
         float w[V], b[V];
-        f.load(row + c);
+        f.load_cached(row + c);
         f.get(v);
 #pragma unroll
         for (int i = 0; i < V; i++) { w[i] = 1.f; b[i] = 0.f; }
@@ -95,8 +95,8 @@ norm_bwd_wide_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restri
     auto take = [&](int c) {  // g = dy * gamma and h of V columns
         Frag<YT, V> fy;
         Frag<XT, V> fx;
-        fy.load(dy + t * lddy + c);
-        fx.load(x + t * ldx + c);
+        fy.load_cached(dy + t * lddy + c);
+        fx.load_cached(x + t * ldx + c);
         fy.get(g);
         fx.get(h);
         if (gamma) {

@@ -47,13 +47,15 @@ inline cudaError_t by_types(int32_t a, int32_t b, F f) {
     return b == OMOE_F32 ? f((bf16 *)nullptr, (float *)nullptr) : f((bf16 *)nullptr, (bf16 *)nullptr);
 }
 
-// V consecutive elements of a row as they lie in memory: 8 (16 bytes of bf16, 32 of fp32) or 1.
+// V consecutive elements of a row as they lie in memory: 8 (16 bytes of bf16, 32 of fp32) or 1.  load() is for what is read once,
+// load_cached() for what is read again and not written by the kernel.
 template <typename T, int V>
 struct Frag;
 template <>
 struct Frag<__nv_bfloat16, 8> {
     uint4 r;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void load_cached(const __nv_bfloat16 *p) { r = __ldg(reinterpret_cast<const uint4 *>(p)); }
     __device__ __forceinline__ void store(__nv_bfloat16 *p) const { *reinterpret_cast<uint4 *>(p) = r; }
     __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(r, v); }
@@ -102,6 +104,7 @@ template <>
 struct Frag<__nv_bfloat16, 1> {
     __nv_bfloat16 r;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = __ldcs(p); }
+    __device__ __forceinline__ void load_cached(const __nv_bfloat16 *p) { r = __ldg(p); }
     __device__ __forceinline__ void store(__nv_bfloat16 *p) const { *p = r; }
     __device__ __forceinline__ void zero() { r = __float2bfloat16_rn(0.f); }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = __bfloat162float(r); }
