@@ -183,7 +183,8 @@ norm_cols_kernel(const YT *__restrict__ dy, int64_t lddy, const XT *__restrict__
 // ---- rows that fit a block's registers ----------------------------------------------------------------------------
 //
 // A block of B threads works on B / G rows at a time: G threads hold a row, P vectors of V elements each, and walk the rows of the
-// grid with a stride.  Rows arrive in a ring of S stages in shared memory by asynchronous copies that a warp makes for
+// grid with a stride.  The forms for few threads (FEW) take for a row the whole warps that it needs instead, and as many rows as then
+// fit the block: few_forward and few_backward.  Rows arrive in a ring of S stages in shared memory by asynchronous copies that a warp makes for
 // its own columns alone, so the ring needs no block barrier, and the loads of the next S - 1 rows are on their way while a
 // row is reduced.  The reductions are what threads of a row meet for: warp shuffles, then one named barrier each.
 // Bound by the issue of instructions before it is by HBM, hence pairs of values in the packed fp32 instructions, sums that
@@ -253,8 +254,8 @@ struct Ahead {
     uint32_t first, second, put;  // this thread's pieces, and where it puts what it copies
     int col;                      // the first column it copies
     // vectors behind the row's end are zeros in every stage from the start
-    __device__ __forceinline__ Ahead(uint32_t ring, int d) {
-        const int lane = threadIdx.x & 31, in_row = threadIdx.x % G;
+    __device__ __forceinline__ Ahead(uint32_t ring, int d, int in_row) {
+        const int lane = threadIdx.x & 31;
         const uint32_t warp = ring + (threadIdx.x - lane) * 16 * kPieces;
         const int swap = kPieces == 2 ? lane >> 2 & 1 : 0;
         first = warp + (lane * kPieces ^ swap) * 16;
@@ -302,7 +303,7 @@ struct Ahead<T, B, 1, G, P, S> {
     static constexpr int kStage = 0;
     Frag<T, 1> next[P];
     int col;
-    __device__ __forceinline__ Ahead(uint32_t, int) : col(threadIdx.x % G) {
+    __device__ __forceinline__ Ahead(uint32_t, int, int in_row) : col(in_row) {
 #pragma unroll
         for (int p = 0; p < P; p++) next[p].zero();
     }
@@ -325,11 +326,11 @@ struct Ahead<T, B, 1, G, P, S> {
 
 // What a thread holds of a row, in groups of pairs that are read and stored together: a vector each (V = 8), or all of its
 // single elements (V = 1).
-template <int V, int G, int P>
+template <int V, int G, int P, bool FEW>
 struct Part {
     static constexpr int kGroups = V == 8 ? P : 1, kPairs = V == 8 ? 4 : P / 2;
-    int d;
-    __device__ __forceinline__ int in_row() const { return threadIdx.x % G; }
+    int d, mine;  // the row's width, the thread's number in the row
+    __device__ __forceinline__ int in_row() const { return FEW ? mine : threadIdx.x % G; }
     __device__ __forceinline__ int col(int q) const { return V == 8 ? (q * G + in_row()) * 8 : in_row(); }
     __device__ __forceinline__ bool has(int q) const { return col(q) < d; }
     // single elements: zeros in place of what lies behind the row's end
@@ -391,8 +392,8 @@ constexpr int kFwdBlocks = 1024 / kFwdBlock<G>;
 template <typename XT, int V, int G, int P>
 constexpr int kBwdBlocks = P > 4 || (V == 8 && P > 1) ? 1 : 1024 / kBwdBlock<XT, V, G, P>;
 // Rows that a forward block's threads take at a time.  Where many threads share a row of bf16, two rows share their barriers and
-// shuffles (16384 x 4096: 44 us, one by one 50; 40000 x 1536: 44 and 55); fp32 is bound by HBM either way, and narrower rows are
-// faster one by one (65536 x 1024: 49 us and 45).
+// shuffles (16384 x 4096: 44 us, one by one 50; 40000 x 1536 on 256 threads a row: 44 and 55); fp32 is bound by HBM either way, and
+// narrower rows are faster one by one (65536 x 1024: 49 us and 45).
 template <typename XT, int V, int G>
 constexpr int kFwdRows = V == 8 && G >= 256 && sizeof(XT) == 2 ? 2 : 1;
 // Stages that fit a block's share of shared memory.  Forward two beside those of two goes (16384 x 4096 of bf16 with four 45.3 us, with six
@@ -408,24 +409,44 @@ template <typename XT, typename YT, int V, int G, int P>
 constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>,
                                                   sizeof(XT) == 2 ? 3 : G == 512 ? 2 : 4);
 
-template <int B, int G>
-__device__ __forceinline__ void row_barrier() {
-    static_assert(B == G || G == 32 || B / G < 16, "a named barrier for every row");
-    if constexpr (G == B) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / G + 1), "n"(G) : "memory");
-}
+// The threads of a block, by row.
+template <int B, int G, bool FEW>
+struct Block {
+    // rows at a time: B / G, or as many as a block can have of at least G / 2 + 32 threads each
+    static constexpr int kRows = FEW ? 2 * B / (G + 64) : B / G;
+    static_assert(G == 32 || kRows == 1 || kRows < 16, "a named barrier for every row");
+    static constexpr int kWords = kRows * 2 * (G / 32);  // two for every warp that a row can have
+    int row_threads;
+    __device__ __forceinline__ int threads() const { return FEW ? row_threads : G; }
+    __device__ __forceinline__ int all() const { return FEW ? (int)blockDim.x : B; }
+    __device__ __forceinline__ int rows() const { return FEW ? all() / row_threads : B / G; }
+    __device__ __forceinline__ int in_row() const { return threadIdx.x % threads(); }
+    __device__ __forceinline__ unsigned warp() const { return FEW ? (unsigned)in_row() >> 5 : threadIdx.x % G >> 5; }
+    __device__ __forceinline__ void row_barrier() const {
+        if constexpr (G == B) __syncthreads();
+        else if constexpr (FEW) asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / row_threads + 1), "r"(row_threads) : "memory");
+        else asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / G + 1), "n"(G) : "memory");
+    }
+    // the words of warps that the rows do not have stay zero
+    __device__ __forceinline__ void clear(float (&words)[2][kWords]) const {
+        if constexpr (FEW) {
+            for (int i = threadIdx.x; i < 2 * kWords; i += all()) words[i / kWords][i % kWords] = 0.f;
+            __syncthreads();
+        }
+    }
+};
 
-// The sum of v over the G threads of a row, in all of them.  s: G / 32 words of this row; between two uses the
-// threads of the row have to meet at another barrier.
-template <int B, int G>
-__device__ __forceinline__ float row_sum(float v, float *s) {
+// The sum of v over the threads of a row, in all of them.  s: words of this row; between two uses the threads of the row
+// have to meet at another barrier.
+template <int B, int G, bool FEW>
+__device__ __forceinline__ float row_sum(float v, float *s, const Block<B, G, FEW> &block) {
     constexpr int W = G / 32;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     if constexpr (W > 1) {
         const int lane = threadIdx.x & 31;
-        if (lane == 0) s[(threadIdx.x % G) >> 5] = v;
-        row_barrier<B, G>();
+        if (lane == 0) s[block.warp()] = v;
+        block.row_barrier();
         v = s[lane & (W - 1)];
 #pragma unroll
         for (int m = W / 2; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
@@ -433,9 +454,9 @@ __device__ __forceinline__ float row_sum(float v, float *s) {
     return v;
 }
 
-// Two sums at once, 2 * (G / 32) words: after one exchange the lower half of a warp adds up a and the upper half b.
-template <int B, int G>
-__device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
+// Two sums at once: after one exchange the lower half of a warp adds up a and the upper half b.
+template <int B, int G, bool FEW>
+__device__ __forceinline__ void row_sums(float &a, float &b, float *s, const Block<B, G, FEW> &block) {
     constexpr int W = G / 32;
     const int lane = threadIdx.x & 31, half = lane >> 4;
     float v = half ? b : a;
@@ -443,8 +464,8 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     if constexpr (W > 1) {
-        if ((lane & 15) == 0) s[half * W + ((threadIdx.x % G) >> 5)] = v;
-        row_barrier<B, G>();
+        if ((lane & 15) == 0) s[half * W + block.warp()] = v;
+        block.row_barrier();
         v = s[half * W + (lane & (W - 1) & 15)];
         if constexpr (W == 32) v += s[half * W + 16 + (lane & 15)];
 #pragma unroll
@@ -455,9 +476,9 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *s) {
 }
 
 // gamma or beta of this thread's columns: in registers where a thread holds 8 elements, else from cache for every row.
-template <int V, int G, int P>
+template <int V, int G, int P, bool FEW>
 struct Param {
-    using Mine = Part<V, G, P>;
+    using Mine = Part<V, G, P, FEW>;
     static constexpr bool kKept = P * V <= 8;
     const float *p;
     float missing;
@@ -475,24 +496,26 @@ struct Param {
     }
 };
 
-template <typename XT, typename YT, int V, int G, int P>
+template <typename XT, typename YT, int V, int G, int P, bool FEW>
 __global__ void __launch_bounds__(kFwdBlock<G>, kFwdBlocks<G>)
 norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
-            YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d) {
-    using Mine = Part<V, G, P>;
+            YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d, int row_threads) {
+    using Mine = Part<V, G, P, FEW>;
     constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G>, Q = Mine::kGroups, N = Mine::kPairs;
     static_assert(S >= 2 * R, "rows are read from some stages while others fill");
     extern __shared__ __align__(16) char sm[];
-    __shared__ float s_sum[2][2 * B / 32];
-    const int group = threadIdx.x / G;
-    const int step = gridDim.x * (B / G);
-    const Mine part = {d};
-    Ahead<XT, B, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d);
+    __shared__ float s_sum[2][Block<B, G, FEW>::kWords];
+    const int group = FEW ? threadIdx.x / row_threads : threadIdx.x / G;
+    const int step = gridDim.x * (FEW ? blockDim.x / row_threads : B / G);
+    const Block<B, G, FEW> block{row_threads};
+    block.clear(s_sum);
+    const Mine part = {d, block.in_row()};
+    Ahead<XT, B, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d, part.in_row());
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, G, P> scale(gamma, part, 1.f), shift(beta, part, 0.f);
-    int t = blockIdx.x * (B / G) + group;  // T and the rows of 2 S strides stay below 2^31: kRowsMax
+    const Param<V, G, P, FEW> scale(gamma, part, 1.f), shift(beta, part, 0.f);
+    int t = blockIdx.x * (FEW ? blockDim.x / row_threads : B / G) + group;  // T and the rows of 2 S strides stay below 2^31: kRowsMax
     int next = t;  // the row to fetch
     x += ahead.col;
     y += part.col(0);
@@ -523,8 +546,8 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
                 for (int i = 0; i < N; i++) pair = add2(pair, v[r][q][i]);
             sum[r] = both(pair);
         }
-        if constexpr (R == 2) row_sums<B, G>(sum[0], sum[1], s_mean);
-        else sum[0] = row_sum<B, G>(sum[0], s_mean);
+        if constexpr (R == 2) row_sums(sum[0], sum[1], s_mean, block);
+        else sum[0] = row_sum(sum[0], s_mean, block);
 #pragma unroll
         for (int r = 0; r < R; r++) {
             mean[r] = sum[r] * inv;
@@ -541,8 +564,8 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
             }
             sum[r] = both(pair);
         }
-        if constexpr (R == 2) row_sums<B, G>(sum[0], sum[1], s_var);
-        else sum[0] = row_sum<B, G>(sum[0], s_var);
+        if constexpr (R == 2) row_sums(sum[0], sum[1], s_var, block);
+        else sum[0] = row_sum(sum[0], s_var, block);
 #pragma unroll
         for (int r = 0; r < R; r++) rstd[r] = rsqrtf(fmaf(sum[r], inv, eps));
         if (part.in_row() == 0) {
@@ -584,33 +607,35 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
 
 // The column sums of dy * h and dy stay in registers over all of a block's rows; each block leaves them in `partial`.  With
 // several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
-template <typename XT, typename YT, int V, int G, int P>
+template <typename XT, typename YT, int V, int G, int P, bool FEW>
 __global__ void __launch_bounds__(kBwdBlock<XT, V, G, P>, kBwdBlocks<XT, V, G, P>)
 norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma,
                 const float *__restrict__ mean, const float *__restrict__ rstd, XT *__restrict__ dx, uint32_t dx_pitch,
-                float *__restrict__ partial, int T, int d) {
-    using Mine = Part<V, G, P>;
+                float *__restrict__ partial, int T, int d, int row_threads) {
+    using Mine = Part<V, G, P, FEW>;
     constexpr int B = kBwdBlock<XT, V, G, P>, S = kBwdStages<XT, YT, V, G, P>, Q = Mine::kGroups, N = Mine::kPairs;
     constexpr bool kAgain = Q > 1;
     static_assert(S >= 2, "a row is read from one stage while another one fills");
     extern __shared__ __align__(16) char sm[];
-    __shared__ float s_sum[2][2 * B / 32];
-    const int group = threadIdx.x / G;
-    const int step = gridDim.x * (B / G);
-    const Mine part = {d};
+    __shared__ float s_sum[2][Block<B, G, FEW>::kWords];
+    const int group = FEW ? threadIdx.x / row_threads : threadIdx.x / G;
+    const int step = gridDim.x * (FEW ? blockDim.x / row_threads : B / G);
+    const Block<B, G, FEW> block{row_threads};
+    block.clear(s_sum);
+    const Mine part = {d, block.in_row()};
     f2 dg[Q][N], db[Q][N];
 #pragma unroll
     for (int q = 0; q < Q; q++)
 #pragma unroll
         for (int i = 0; i < N; i++) dg[q][i] = db[q][i] = 0ull;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm);
-    Ahead<XT, B, V, G, P, S> ahead_x(ring, d);
-    Ahead<YT, B, V, G, P, S> ahead_y(ring + S * Ahead<XT, B, V, G, P, S>::kStage, d);
+    Ahead<XT, B, V, G, P, S> ahead_x(ring, d, part.in_row());
+    Ahead<YT, B, V, G, P, S> ahead_y(ring + S * Ahead<XT, B, V, G, P, S>::kStage, d, part.in_row());
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, G, P> scale(gamma, part, 1.f);
-    int t = blockIdx.x * (B / G) + group, next = t;
+    const Param<V, G, P, FEW> scale(gamma, part, 1.f);
+    int t = blockIdx.x * (FEW ? blockDim.x / row_threads : B / G) + group, next = t;
     x += ahead_x.col;
     dy += ahead_y.col;
     dx += part.col(0);
@@ -629,7 +654,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
         m = mean[t];
         r = rstd[t];
     }
-    auto row = [&](int stage, int odd) {
+    auto row = [&](int stage, int turn) {
         f2 h[Q][N], g[Q][N], sum_g = 0ull, sum_gh = 0ull;
         const f2 minus = pack2(-m, -m), rr = pack2(r, r);
         if (t + step < T) {
@@ -661,7 +686,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
             }
         }
         float mg = both(sum_g), mh = both(sum_gh);
-        row_sums<B, G>(mg, mh, s_sum[odd] + group * (2 * G / 32));
+        row_sums(mg, mh, s_sum[turn] + group * (2 * G / 32), block);
         const f2 less = pack2(-mg * inv, -mg * inv), slope = pack2(-mh * inv, -mh * inv);
 #pragma unroll
         for (int q = 0; q < Q; q++) {
@@ -702,27 +727,26 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
             part.store(sums + d + part.col(0), q, db[q]);
         }
     } else {
-        constexpr int W = G * P * V;  // columns a group covers
+        const int cols = block.threads() * P * V;  // that a row's threads cover
         float *s = reinterpret_cast<float *>(sm);
-        const Mine whole = {W};
         copies_wait<0>();
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < Q; q++)
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int c = V == 8 ? whole.col(q) + 2 * i : whole.in_row() + 2 * i * G, next_c = V == 8 ? 1 : G;
-                float *a = s + group * 2 * W + c, *b = a + W;
+                const int c = V == 8 ? part.col(q) + 2 * i : part.in_row() + 2 * i * G, next_c = V == 8 ? 1 : G;
+                float *a = s + group * 2 * cols + c, *b = a + cols;
                 unpack2(dg[q][i], a[0], a[next_c]);
                 unpack2(db[q][i], b[0], b[next_c]);
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * W; i += B) {
-            const int which = i / W, col = i % W;
+        for (int i = threadIdx.x; i < 2 * cols; i += block.all()) {
+            const int which = i / cols, col = i % cols;
             if (col >= d) continue;
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < B / G; q++) sum += s[(q * 2 + which) * W + col];
+            for (int q = 0; q < block.rows(); q++) sum += s[(q * 2 + which) * cols + col];
             sums[which * d + col] = sum;
         }
     }
@@ -794,6 +818,18 @@ bool by_width(bool vec, int d, F f) {
     return true;
 }
 
+// The whole warps that a row of width d needs where a thread holds one vector, in threads.
+int few_threads(int d) { return ceil_div(d, 256) * 32; }
+// Which kernels have a form for few threads.  Forward it gains wherever y is bf16 (20000 x 2224 from fp32: 60 us, with few threads 43;
+// from bf16 41 and 31; 40000 x 1536 from bf16 44 and 40).  Rows of fp32 results are slower several at a time (40000 x 1200: 64 and 72), so
+// there only those of a whole block have it (10000 x 4352: 73 and 63).
+template <typename YT, int V, int G, int P>
+constexpr bool few_forward = V == 8 && P == 1 && G >= 128 && (sizeof(YT) == 2 || G == 1024);
+// Backward, where more rows fit a block: for bf16 x (40000 x 1200 of bf16: 68 us, with few threads 54; 20000 x 2224: 68 and 54), and for
+// fp32 x with bf16 dy in the middle (40000 x 1200: 103 and 87, but 60000 x 640: 67 and 71); not with both fp32 (40000 x 1200: 90 and 96).
+template <typename XT, typename YT, int V, int G, int P>
+constexpr bool few_backward = V == 8 && P == 1 && G >= 128 && G < kBwdBlock<XT, V, G, P> && (sizeof(XT) == 2 || (sizeof(YT) == 2 && G == 256));
+
 template <typename K>
 cudaError_t allow_smem(K kern, size_t bytes, PerDeviceOnce &once) {
     bool *done = once.slot();
@@ -837,14 +873,21 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
                      [&](auto v, auto g, auto p) {
                          constexpr int V = decltype(v)::value, G = decltype(g)::value, P = decltype(p)::value;
                          constexpr size_t smem = kFwdStages<XT, V, G, P> * Ahead<XT, kFwdBlock<G>, V, G, P, 2>::kStage;
+                         auto launch = [&](auto kern, PerDeviceOnce &once, int row) {
+                             e = allow_smem(kern, smem, once);
+                             if (e != cudaSuccess) return;
+                             const int at_once = kFwdBlock<G> / row, threads = at_once * row;
+                             const int blocks = ceil_div(T, at_once), most = 1024 / threads * sms;
+                             e = launch_ex(kern, dim3(blocks < most ? blocks : most), dim3(threads), smem, s, ops_pdl(),
+                                           static_cast<const XT *>(x_dev), (uint32_t)(ldx * sizeof(XT)), gamma_dev, beta_dev, eps,
+                                           static_cast<YT *>(y_dev), (uint32_t)(ldy * sizeof(YT)), mean_dev, rstd_dev, T, d, row);
+                         };
                          static PerDeviceOnce once;
-                         e = allow_smem(norm_kernel<XT, YT, V, G, P>, smem, once);
-                         if (e != cudaSuccess) return;
-                         const int blocks = ceil_div(T, kFwdBlock<G> / G), most = kFwdBlocks<G> * sms;
-                         e = launch_ex(norm_kernel<XT, YT, V, G, P>, dim3(blocks < most ? blocks : most), dim3(kFwdBlock<G>), smem, s, ops_pdl(),
-                                       static_cast<const XT *>(x_dev), (uint32_t)(ldx * sizeof(XT)), gamma_dev, beta_dev, eps, static_cast<YT *>(y_dev),
-                                       (uint32_t)(ldy * sizeof(YT)),
-                                       mean_dev, rstd_dev, T, d);
+                         if constexpr (few_forward<YT, V, G, P>) {
+                             static PerDeviceOnce once_few;
+                             if (few_threads(d) < G) return launch(norm_kernel<XT, YT, V, G, P, true>, once_few, few_threads(d));
+                         }
+                         launch(norm_kernel<XT, YT, V, G, P, false>, once, G);
                      }))
             return e;
         auto wide = [&](auto kern) {
@@ -901,17 +944,25 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
                                       constexpr size_t ring = S * (Ahead<XT, B, V, G, P, S>::kStage + Ahead<YT, B, V, G, P, S>::kStage);
                                       constexpr size_t join = G < B ? 2 * B * P * V * sizeof(float) : 0;
                                       constexpr size_t smem = ring > join ? ring : join;
+                                      auto launch = [&](auto kern, PerDeviceOnce &once, int row) {
+                                          e = allow_smem(kern, smem, once);
+                                          if (e != cudaSuccess) return;
+                                          const int at_once = B / row, blocks = ceil_div(T, at_once);
+                                          int most = kBwdBlocks<XT, V, G, P> * sms;
+                                          most = most < kBwdBlocksMax ? most : kBwdBlocksMax;
+                                          sums = blocks < most ? blocks : most;
+                                          e = launch_ex(kern, dim3(sums), dim3(at_once * row), smem, s, ops_pdl(), g,
+                                                        (uint32_t)(lddy * sizeof(YT)), in, (uint32_t)(ldx * sizeof(XT)), gamma_dev, mean_dev,
+                                                        rstd_dev, static_cast<XT *>(dx_dev), (uint32_t)(lddx * sizeof(XT)),
+                                                        params ? partial : nullptr, T, d, row);
+                                      };
                                       static PerDeviceOnce once;
-                                      e = allow_smem(norm_bwd_kernel<XT, YT, V, G, P>, smem, once);
-                                      if (e != cudaSuccess) return;
-                                      const int blocks = ceil_div(T, B / G);
-                                      int most = kBwdBlocks<XT, V, G, P> * sms;
-                                      most = most < kBwdBlocksMax ? most : kBwdBlocksMax;
-                                      sums = blocks < most ? blocks : most;
-                                      e = launch_ex(norm_bwd_kernel<XT, YT, V, G, P>, dim3(sums), dim3(B), smem, s, ops_pdl(), g,
-                                                    (uint32_t)(lddy * sizeof(YT)), in, (uint32_t)(ldx * sizeof(XT)), gamma_dev, mean_dev,
-                                                    rstd_dev, static_cast<XT *>(dx_dev), (uint32_t)(lddx * sizeof(XT)),
-                                                    params ? partial : nullptr, T, d);
+                                      if constexpr (few_backward<XT, YT, V, G, P>) {
+                                          static PerDeviceOnce once_few;
+                                          if (B / few_threads(d) > B / G)
+                                              return launch(norm_bwd_kernel<XT, YT, V, G, P, true>, once_few, few_threads(d));
+                                      }
+                                      launch(norm_bwd_kernel<XT, YT, V, G, P, false>, once, G);
                                   }
                               }) && (e != cudaSuccess || sums > 0)) {
             if (e != cudaSuccess || !params) return e;
