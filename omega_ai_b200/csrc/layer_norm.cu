@@ -394,8 +394,8 @@ constexpr int kBwdBlocks = P > 4 || (V == 8 && P > 1) ? 1 : 1024 / kBwdBlock<XT,
 // Rows that a forward block's threads take at a time.  Where many threads share a row of bf16, two rows share their barriers and
 // shuffles (16384 x 4096: 44 us, one by one 50; 40000 x 1536 on 256 threads a row: 44 and 55); fp32 is bound by HBM either way, and
 // narrower rows are faster one by one (65536 x 1024: 49 us and 45).
-template <typename XT, int V, int G>
-constexpr int kFwdRows = V == 8 && G >= 256 && sizeof(XT) == 2 ? 2 : 1;
+template <typename XT, int V, int G, int P>
+constexpr int kFwdRows = V == 8 && G >= 256 && (P == 1 || G == 1024) && sizeof(XT) == 2 ? 2 : 1;
 // Stages that fit a block's share of shared memory.  Forward two beside those of two goes (16384 x 4096 of bf16 with four 45.3 us, with six
 // 43.9).  Backward three for bf16 (with four 65536 x 256 takes 23.3 us, 22.4 with three), four for fp32, and two where two blocks
 // of long fp32 rows share an SM (x 4096 to bf16, 8192 to 30011 rows: 52 to 186 us, with four 57 to 215).
@@ -404,7 +404,7 @@ constexpr int stages(int stage_bytes, int blocks, int most) {
     return fit > most ? most : fit;
 }
 template <typename XT, int V, int G, int P>
-constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, 2 + 2 * kFwdRows<XT, V, G>);
+constexpr int kFwdStages = V == 1 ? 2 : stages(kFwdBlock<G> * P * V * (int)sizeof(XT), kFwdBlocks<G>, 2 + 2 * kFwdRows<XT, V, G, P>);
 template <typename XT, typename YT, int V, int G, int P>
 constexpr int kBwdStages = V == 1 ? 2 : stages(kBwdBlock<XT, V, G, P> * P * V * (int)(sizeof(XT) + sizeof(YT)), kBwdBlocks<XT, V, G, P>,
                                                   sizeof(XT) == 2 ? 3 : G == 512 ? 2 : 4);
@@ -475,21 +475,20 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *s, const Blo
     b = __shfl_sync(0xffffffffu, v, 16);
 }
 
-// gamma or beta of this thread's columns: in registers where a thread holds 8 elements, else from cache for every row.
-template <int V, int G, int P, bool FEW>
+// gamma or beta of this thread's columns: in registers (KEPT), or from cache for every row.
+template <int V, int G, int P, bool FEW, bool KEPT>
 struct Param {
     using Mine = Part<V, G, P, FEW>;
-    static constexpr bool kKept = P * V <= 8;
     const float *p;
     float missing;
-    f2 kept[kKept ? Mine::kGroups : 1][Mine::kPairs];
+    f2 kept[KEPT ? Mine::kGroups : 1][Mine::kPairs];
     __device__ __forceinline__ Param(const float *from, const Mine &part, float absent) : p(from), missing(absent) {
-        if constexpr (kKept)
+        if constexpr (KEPT)
 #pragma unroll
             for (int q = 0; q < Mine::kGroups; q++) part.load(p, q, missing, kept[q]);
     }
     __device__ __forceinline__ void get(const Mine &part, int q, f2 (&v)[Mine::kPairs]) const {
-        if constexpr (kKept) {
+        if constexpr (KEPT) {
 #pragma unroll
             for (int i = 0; i < Mine::kPairs; i++) v[i] = kept[q][i];
         } else part.load(p, q, missing, v);
@@ -501,7 +500,7 @@ __global__ void __launch_bounds__(kFwdBlock<G>, kFwdBlocks<G>)
 norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
             YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d, int row_threads) {
     using Mine = Part<V, G, P, FEW>;
-    constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G>, Q = Mine::kGroups, N = Mine::kPairs;
+    constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G, P>, Q = Mine::kGroups, N = Mine::kPairs;
     static_assert(S >= 2 * R, "rows are read from some stages while others fill");
     extern __shared__ __align__(16) char sm[];
     __shared__ float s_sum[2][Block<B, G, FEW>::kWords];
@@ -514,7 +513,10 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, G, P, FEW> scale(gamma, part, 1.f), shift(beta, part, 0.f);
+    // Kept also where a thread has two vectors (8192 x 8192 of bf16 43 us, read from cache 55), but on 1024 threads only from fp32 to bf16
+    // (4096 x 16384: 65 and 76; from bf16 60 and 57, fp32 to fp32 95 and 90).
+    constexpr bool kKept = P * V <= 8 || (V == 8 && (G < 1024 || (sizeof(XT) == 4 && sizeof(YT) == 2)));
+    const Param<V, G, P, FEW, kKept> scale(gamma, part, 1.f), shift(beta, part, 0.f);
     int t = blockIdx.x * (FEW ? blockDim.x / row_threads : B / G) + group;  // T and the rows of 2 S strides stay below 2^31: kRowsMax
     int next = t;  // the row to fetch
     x += ahead.col;
@@ -634,7 +636,7 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
     const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
-    const Param<V, G, P, FEW> scale(gamma, part, 1.f);
+    const Param<V, G, P, FEW, P * V <= 8> scale(gamma, part, 1.f);
     int t = blockIdx.x * (FEW ? blockDim.x / row_threads : B / G) + group, next = t;
     x += ahead_x.col;
     dy += ahead_y.col;
@@ -787,14 +789,24 @@ int slices_of(int T, int d, int per_thread, int sms) {
 }
 
 // Calls f with the vector width, threads per row and vectors per thread (integral constants) for rows of width d, or
-// returns false where they do not fit a block's registers.  Vectors: the fewest threads that hold the row with one each, then two.
+// returns false where they do not fit a block's registers.  Vectors: the fewest threads that hold the row with one each, then two, with
+// the exceptions below.
 // Single elements: eight per thread, then sixteen (fewer elements and more threads per row: 20000 x 1001 of bf16 forward 53 us with four on 512
 // threads, 21 with eight on 128, 35 with sixteen on 64).
 template <int N>
 using Int = std::integral_constant<int, N>;
-template <bool BACK, typename F>
-bool by_width(bool vec, int d, F f) {
+template <bool BACK, typename XT, typename YT, typename F>
+bool by_width(bool vec, int T, int d, F f) {
     if (vec) {
+        // Two vectors on half the threads halve the shuffles and barriers; forward that is faster for rows of bf16 from bf16 where
+        // many of them (60000 x 640: 35 us, with two vectors 30; 6000: 5.4 and 5.6) are not too wide (x 896: 41 and 35, 65536 x 1024: 44
+        // and 48), ...
+        if constexpr (!BACK && sizeof(XT) == 2 && sizeof(YT) == 2)
+            if (T >= 8000 && d > 512 && d <= 896) return f(Int<8>(), Int<64>(), Int<2>()), true;
+        // ... and where a row has an SM to itself otherwise and now two share it: to bf16 from bf16 (8192 x 8192: 47 and 43, 8000 x 5120: 33
+        // and 35) and from fp32 (8000 x 5888: 51 and 44, 8192 x 8192: 63 and 68), not to fp32 (8192 x 8192: 82 and 97).
+        if constexpr (!BACK && sizeof(YT) == 2)
+            if (sizeof(XT) == 2 ? d > 5120 && d <= 8192 : d > 4096 && d <= 7168) return f(Int<8>(), Int<512>(), Int<2>()), true;
         if (d <= 256) f(Int<8>(), Int<32>(), Int<1>());
         else if (d <= 512) f(Int<8>(), Int<64>(), Int<1>());
         else if (d <= 1024) f(Int<8>(), Int<128>(), Int<1>());
@@ -869,7 +881,7 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
         using YT = std::remove_pointer_t<decltype(yt)>;
         cudaError_t e = cudaSuccess;
         const bool vec = rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 32) && !misaligned(beta_dev, 32);
-        if (by_width<false>(vec, d,
+        if (by_width<false, XT, YT>(vec, T, d,
                      [&](auto v, auto g, auto p) {
                          constexpr int V = decltype(v)::value, G = decltype(g)::value, P = decltype(p)::value;
                          constexpr size_t smem = kFwdStages<XT, V, G, P> * Ahead<XT, kFwdBlock<G>, V, G, P, 2>::kStage;
@@ -936,7 +948,7 @@ int omoe_layer_norm_backward(const void *dy_dev, int64_t lddy, int32_t dy_dtype,
         cudaError_t e = cudaSuccess;
         int sums = 0;  // column sums in the workspace
         const bool vec = rows_vector(x) && rows_vector(dy) && rows_vector(dx) && !misaligned(gamma_dev, 32);
-        if (T > 0 && by_width<true>(vec, d,
+        if (T > 0 && by_width<true, XT, YT>(vec, T, d,
                               [&](auto v, auto gg, auto p) {
                                   constexpr int V = decltype(v)::value, G = decltype(gg)::value, P = decltype(p)::value;
                                   constexpr int S = kBwdStages<XT, YT, V, G, P>, B = kBwdBlock<XT, V, G, P>;

@@ -152,7 +152,7 @@ def test_no_rows():
 
 @pytest.mark.parametrize("xt,yt", [(BF, BF), (F32, BF), (BF, F32), (F32, F32)])
 @pytest.mark.parametrize("T,d", [(1, 520), (4001, 520), (13, 768), (4001, 1032), (3, 1536), (3001, 1528), (2, 2056), (2500, 2560), (1, 4104),
-                                 (901, 4352), (77, 7000)])
+                                 (901, 4352), (77, 7000), (8100, 648), (8001, 896), (400, 8184)])
 def test_rows_between_powers_of_two(T, d, xt, yt):
     """Rows that leave whole warps of the next power of two idle: fewer threads share a row, several rows a block."""
     test_forward_and_backward(T, d, xt, yt, "packed", "both", 1.0, 0.5)
