@@ -344,6 +344,17 @@ struct Part {
             }
         }
     }
+    // sum + a * b; of single elements only where the row has them (the first half of its threads' elements it always has, but on one warp)
+    __device__ __forceinline__ f2 add_product(int i, f2 a, f2 b, f2 sum) const {
+        if constexpr (V == 1) {
+            if (G == 32 || 4 * i >= P) {
+                float c, e;
+                unpack2(b, c, e);
+                b = pack2(in_row() + 2 * i * G < d ? c : 0.f, in_row() + (2 * i + 1) * G < d ? e : 0.f);
+            }
+        }
+        return fma2(a, b, sum);
+    }
     __device__ __forceinline__ void load(const float *p, int q, float missing, f2 (&v)[kPairs]) const {
 #pragma unroll
         for (int i = 0; i < kPairs; i++) v[i] = pack2(missing, missing);
@@ -609,6 +620,12 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
 
 // The column sums of dy * h and dy stay in registers over all of a block's rows; each block leaves them in `partial`.  With
 // several vectors per thread the row itself does not fit beside them and is read from its stage again for dx.
+// Columns that the row does not have must not meet the others in the sum of g * h: they have g = 0, but h = (0 - mean) * rstd, and
+// where that is infinite (a row of equal numbers 2^100, eps 1e-30) the product is NaN.  At the limit of the registers every form needs a way of its
+// own: a thread with one vector behind the row's end has mean = rstd = 0 (kNone); in the forms for few threads, where these loads diverge
+// (20000 x 2224 of bf16 54 us, with them 60), it adds nothing in the end; of several vectors those that may be missing (the second half: by_width)
+// have rstd = 0; single elements are masked in the product.  Against sums that take them in: 16384 x 4096 of bf16 68 us both, 65536 x 264 34 and 33,
+// 4096 x 16384 from fp32 146 and 144, of bf16 113 and 116.
 template <typename XT, typename YT, int V, int G, int P, bool FEW>
 __global__ void __launch_bounds__(kBwdBlock<XT, V, G, P>, kBwdBlocks<XT, V, G, P>)
 norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma,
@@ -651,15 +668,16 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
     };
 #pragma unroll
     for (int i = 0; i < S - 1; i++) fetch(i);
+    constexpr bool kNone = V == 8 && P == 1 && !FEW;
     float m = 0.f, r = 0.f;
-    if (t < T) {
+    if (t < T && (!kNone || part.has(0))) {
         m = mean[t];
         r = rstd[t];
     }
     auto row = [&](int stage, int turn) {
         f2 h[Q][N], g[Q][N], sum_g = 0ull, sum_gh = 0ull;
         const f2 minus = pack2(-m, -m), rr = pack2(r, r);
-        if (t + step < T) {
+        if (t + step < T && (!kNone || part.has(0))) {
             m = mean[t + step];
             r = rstd[t + step];
         }
@@ -679,15 +697,16 @@ norm_bwd_kernel(const YT *__restrict__ dy, uint32_t dy_pitch, const XT *__restri
             scale.get(part, q, w);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                h[q][i] = mul2(add2(h[q][i], minus), rr);
+                h[q][i] = mul2(add2(h[q][i], minus), kAgain && 2 * q >= P && !part.has(q) ? 0ull : rr);
                 dg[q][i] = fma2(g[q][i], h[q][i], dg[q][i]);
                 db[q][i] = add2(db[q][i], g[q][i]);
                 g[q][i] = mul2(g[q][i], w[i]);
                 sum_g = add2(sum_g, g[q][i]);
-                sum_gh = fma2(g[q][i], h[q][i], sum_gh);
+                sum_gh = part.add_product(i, g[q][i], h[q][i], sum_gh);
             }
         }
         float mg = both(sum_g), mh = both(sum_gh);
+        if (FEW && !part.has(0)) mh = 0.f;
         row_sums(mg, mh, s_sum[turn] + group * (2 * G / 32), block);
         const f2 less = pack2(-mg * inv, -mg * inv), slope = pack2(-mh * inv, -mh * inv);
 #pragma unroll

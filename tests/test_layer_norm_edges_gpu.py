@@ -1,0 +1,54 @@
+"""Layer norm where single rows or columns can go wrong, against the formulas in 64 bits.
+
+Bounds of the backward pass as in test_layer_norm_gpu.py, with u = 2^-24 and D = d / 32 + 40.  Here mean is a number of x's type, so
+x - mean carries one rounding and h two: with H = |h| (1 + 2 u)
+  sums        means of g and g h are off by (D + 4) u of the means of their terms' magnitudes, the second with h's two roundings
+  dx          rstd (both means' errors, the second times H, + 8 u (|g| + |mean g| + |h mean gh|)), and half a step of its type
+  dgamma      (T / 8 + 80) u of the sum over the rows of |dy| H."""
+import pytest
+import torch
+from test_layer_norm_gpu import BF, F32, HALF, U, rows
+
+pytestmark = pytest.mark.gpu
+
+# widths that fill the threads of a row and widths that leave some without a column: one vector per thread, the forms for few
+# threads (520 .. 7000), several vectors, rows of any width; then single elements
+WIDTHS = [(d, "packed") for d in (8, 64, 256, 264, 512, 520, 1024, 1032, 1536, 2048, 2056, 4096, 4104, 7000, 8192, 8200, 16384, 16392)]
+WIDTHS += [(d, "odd") for d in (1, 7, 57, 201, 401, 1001, 1024, 2047, 4095, 8191, 9001)]
+
+
+@pytest.mark.parametrize("xt,yt", [(BF, BF), (F32, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("d,layout", WIDTHS)
+def test_backward_of_rows_whose_mean_times_rstd_overflows(d, layout, xt, yt):
+    """A row of equal numbers v has h = 0 and a finite gradient, also where v * rstd leaves fp32."""
+    from omega_ai_b200 import layer_norm_backward
+
+    T = 37
+    x, _ = rows(T, d, xt, layout, 1)
+    dy, _ = rows(T, d, yt, layout, 2)
+    gamma = 1 + 0.3 * torch.randn(d, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    mean, rstd = torch.zeros(T, device="cuda"), torch.ones(T, device="cuda")
+    for t, v in ((0, 2.0 ** 100), (5, -(2.0 ** 100)), (20, 2.0 ** 110), (T - 1, 2.0 ** 100)):
+        x[t], mean[t], rstd[t] = v, v, 1e15  # of eps = 1e-30
+    dx, dgamma, dbeta = layer_norm_backward(dy, x, gamma, mean, rstd)
+    D = d / 32 + 40
+    m, r = mean.double().unsqueeze(1), rstd.double().unsqueeze(1)
+    g, h = dy.double() * gamma.double(), (x.double() - m) * r
+    H = h.abs() * (1 + 2 * U)
+    mg, mh = g.mean(1, keepdim=True), (g * h).mean(1, keepdim=True)
+    mg_off, mh_off = (D + 4) * U * g.abs().mean(1, keepdim=True), (D + 6) * U * (g.abs() * H).mean(1, keepdim=True)
+    ref = r * (g - mg - h * mh)
+    off = r * (mg_off + H * mh_off + 8 * U * (g.abs() + mg.abs() + H * mh.abs()))
+    assert ((dx.double() - ref).abs() <= off * 1.01 + HALF[xt] * (ref.abs() + off)).all()
+    n = (T / 8 + 80) * U
+    assert ((dgamma.double() - (dy.double() * h).sum(0)).abs() <= n * (dy.double().abs() * H).sum(0)).all()
+    assert ((dbeta.double() - dy.double().sum(0)).abs() <= n * dy.double().abs().sum(0)).all()
+
+    # rows with an infinity or a NaN: none of it leaves the row but for the column sums of dy * h
+    bad = x.clone()
+    bad[3, 0], bad[T - 2, d - 1] = float("inf"), float("nan")
+    mean[3], rstd[3], mean[T - 2], rstd[T - 2] = float("inf"), float("nan"), float("nan"), float("nan")
+    dx2, _, dbeta2 = layer_norm_backward(dy, bad, gamma, mean, rstd)
+    others = [t for t in range(T) if t not in (3, T - 2)]
+    assert torch.equal(dx2[others], dx[others]) and torch.equal(dbeta2, dbeta)
+    assert dx2[3].isnan().all() and dx2[T - 2].isnan().all()
