@@ -8,6 +8,9 @@
 // whose offset is large against their spread.  All sums are fp32 in a fixed order.
 #include "ops.cuh"
 
+#include <float.h>
+#include <math.h>
+
 namespace omoe {
 
 namespace {
@@ -506,10 +509,23 @@ struct Param {
     }
 };
 
+// 1 / d in two parts.  A sum times 1 / d rounded once is off by up to two roundings of the quotient: where d * fl(1 / d) is not 1 (d = 328), a row
+// of equal numbers 1024 gets a mean of 1023.99994 and y = 0.019 instead of 0.  With both parts the quotient is rounded once but for 2^-48 of it.
+// `high` lies below 1 / d and `low` is positive, so that an infinite sum keeps its infinite mean.
+struct Inverse {
+    float nearest, high, low;
+    explicit Inverse(int d) : nearest(1.f / (float)d), high(nearest) {
+        if ((double)high * d > 1.0) high = nextafterf(high, 0.f);  // exact in 64 bits
+        low = fmaxf((float)(1.0 / d - (double)high), FLT_MIN);
+    }
+    __device__ __forceinline__ float mean(float sum) const { return fmaf(sum, high, sum * low); }
+};
+
 template <typename XT, typename YT, int V, int G, int P, bool FEW>
 __global__ void __launch_bounds__(kFwdBlock<G>, kFwdBlocks<G>)
 norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
-            YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d, int row_threads) {
+            YT *__restrict__ y, uint32_t y_pitch, float *__restrict__ mean_out, float *__restrict__ rstd_out, int T, int d, Inverse inv,
+            int row_threads) {
     using Mine = Part<V, G, P, FEW>;
     constexpr int B = kFwdBlock<G>, S = kFwdStages<XT, V, G, P>, R = kFwdRows<XT, V, G, P>, Q = Mine::kGroups, N = Mine::kPairs;
     static_assert(S >= 2 * R, "rows are read from some stages while others fill");
@@ -521,7 +537,6 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
     block.clear(s_sum);
     const Mine part = {d, block.in_row()};
     Ahead<XT, B, V, G, P, S> ahead((uint32_t)__cvta_generic_to_shared(sm), d, part.in_row());
-    const float inv = 1.f / (float)d;
     pdl_trigger();
     pdl_wait();
     // Kept also where a thread has two vectors (8192 x 8192 of bf16 43 us, read from cache 55), but on 1024 threads only from fp32 to bf16
@@ -563,7 +578,7 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
         else sum[0] = row_sum(sum[0], s_mean, block);
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            mean[r] = sum[r] * inv;
+            mean[r] = inv.mean(sum[r]);
             const f2 minus = pack2(-mean[r], -mean[r]);
             f2 pair = 0ull;
 #pragma unroll
@@ -580,7 +595,7 @@ norm_kernel(const XT *__restrict__ x, uint32_t x_pitch, const float *__restrict_
         if constexpr (R == 2) row_sums(sum[0], sum[1], s_var, block);
         else sum[0] = row_sum(sum[0], s_var, block);
 #pragma unroll
-        for (int r = 0; r < R; r++) rstd[r] = rsqrtf(fmaf(sum[r], inv, eps));
+        for (int r = 0; r < R; r++) rstd[r] = rsqrtf(fmaf(sum[r], inv.nearest, eps));
         if (part.in_row() == 0) {
 #pragma unroll
             for (int r = 0; r < R; r++)
@@ -895,6 +910,7 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
     const int sms = ops_sm_count();
     if (!sms) return ops_fail(OMOE_ERR_CUDA, fn, "no device");
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    const Inverse inverse(d);
     return ops_launched(by_types(x_dtype, y_dtype, [&](auto *xt, auto *yt) {
         using XT = std::remove_pointer_t<decltype(xt)>;
         using YT = std::remove_pointer_t<decltype(yt)>;
@@ -911,7 +927,7 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
                              const int blocks = ceil_div(T, at_once), most = 1024 / threads * sms;
                              e = launch_ex(kern, dim3(blocks < most ? blocks : most), dim3(threads), smem, s, ops_pdl(),
                                            static_cast<const XT *>(x_dev), (uint32_t)(ldx * sizeof(XT)), gamma_dev, beta_dev, eps,
-                                           static_cast<YT *>(y_dev), (uint32_t)(ldy * sizeof(YT)), mean_dev, rstd_dev, T, d, row);
+                                           static_cast<YT *>(y_dev), (uint32_t)(ldy * sizeof(YT)), mean_dev, rstd_dev, T, d, inverse, row);
                          };
                          static PerDeviceOnce once;
                          if constexpr (few_forward<YT, V, G, P>) {

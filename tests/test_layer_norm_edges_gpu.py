@@ -52,3 +52,34 @@ def test_backward_of_rows_whose_mean_times_rstd_overflows(d, layout, xt, yt):
     others = [t for t in range(T) if t not in (3, T - 2)]
     assert torch.equal(dx2[others], dx[others]) and torch.equal(dbeta2, dbeta)
     assert dx2[3].isnan().all() and dx2[T - 2].isnan().all()
+
+
+@pytest.mark.parametrize("xt,yt", [(BF, BF), (F32, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("T,d,layout", [
+    (9, 41, "packed"), (9, 328, "packed"), (9, 328, "odd"), (40, 656, "packed"), (8000, 656, "packed"), (8000, 776, "packed"), (40, 664, "aligned"),
+    (40, 1312, "packed"), (9, 2624, "odd"), (5, 2624, "packed"), (5, 5248, "packed"), (5, 6560, "packed"), (5, 6560, "odd"), (3, 10496, "packed"),
+    (3, 20992, "packed")])
+def test_rows_of_equal_numbers_where_the_width_has_no_exact_inverse(T, d, layout, xt, yt):
+    """The sum of d times v is exact for v of few bits, so the mean is v and every element is beta, rounded to its type."""
+    from omega_ai_b200 import layer_norm
+
+    values = torch.tensor([1.0, 3.0, -7.5, 255.0, 1024.0, 65536.0, -0.125, 0.0], device="cuda")
+    x, _ = rows(T, d, xt, layout, 1)
+    v = values[torch.arange(T, device="cuda") % len(values)]
+    x.copy_(v.unsqueeze(1).expand(T, d))
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    gamma, beta = torch.randn(d, generator=gen, device="cuda"), torch.randn(d, generator=gen, device="cuda")
+    y, mean, _ = layer_norm(x, gamma, beta, dtype=yt, stats=True)
+    assert torch.equal(mean, v)
+    assert torch.equal(y, beta.to(yt).expand(T, d))
+
+
+def test_means_of_infinite_sums():
+    """A row with an infinity has an infinite mean, one with both or with a NaN none."""
+    from omega_ai_b200 import layer_norm
+
+    for d in (64, 328, 1001, 20000):
+        x = torch.randn(4, d, device="cuda")
+        x[0, d // 2], x[1, 0], x[2, 1], x[2, d - 1], x[3, 3] = float("inf"), -float("inf"), float("inf"), -float("inf"), float("nan")
+        _, mean, _ = layer_norm(x, stats=True)
+        assert mean[0] == float("inf") and mean[1] == -float("inf") and mean[2:].isnan().all()
