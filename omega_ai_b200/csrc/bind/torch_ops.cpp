@@ -127,6 +127,10 @@ T *vec(const OptTensor &t, int64_t n, const char *name, const c10::Device &devic
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const c10::Device &device) {
     return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
+// A caller's tensor was written: autograd has to refuse what saved it before.
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Tensor matrix_or_new(const OptTensor &out, int64_t rows, int64_t d, at::ScalarType type, const c10::Device &device) {
     return out ? *out : fresh({rows, d}, type, device);
 }
@@ -187,6 +191,7 @@ struct TokenSort {
         const Matrix o(to, rows_cap, d, "out", device);
         const omoe_sort p = c();
         check(lib.sort_rows(&p, in.p, in.ld, in.dtype, o.p, o.ld, o.dtype, fits(d, "x"), on.stream));
+        if (out) written(to);
         return to;
     }
     Tensor sort_backward(const Tensor &dxs, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
@@ -197,6 +202,7 @@ struct TokenSort {
         const Matrix o(to, tokens, d, "out", device);
         const omoe_sort p = c();
         check(lib.sort_rows_backward(&p, in.p, in.ld, in.dtype, o.p, o.ld, o.dtype, fits(d, "dxs"), on.stream));
+        if (out) written(to);
         return to;
     }
     Tensor unsort(const Tensor &ys, const OptTensor &weights, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
@@ -208,6 +214,7 @@ struct TokenSort {
         const Matrix o(to, tokens, d, "out", device);
         const omoe_sort p = c();
         check(lib.unsort_rows(&p, in.p, in.ld, in.dtype, w, o.p, o.ld, o.dtype, fits(d, "ys"), on.stream));
+        if (out) written(to);
         return to;
     }
     std::pair<Tensor, OptTensor> unsort_backward(const Tensor &dy, const Tensor &ys, const OptTensor &weights, const OptTensor &out) const {
@@ -223,6 +230,7 @@ struct TokenSort {
         const omoe_sort p = c();
         check(lib.unsort_rows_backward(&p, g.p, g.ld, g.dtype, y.p, y.ld, y.dtype, w, o.p, o.ld, dw ? static_cast<float *>(dw->data_ptr()) : nullptr,
                                        fits(d, "dy"), on.stream));
+        if (out) written(to);
         return {to, dw};
     }
 };
@@ -241,6 +249,7 @@ py::object layer_norm(const Tensor &x, const OptTensor &gamma, const OptTensor &
     if (stats) std::tie(mean, rstd) = two_floats(T, dev);
     check(lib.layer_norm(in.p, in.ld, in.dtype, g, b, (float)eps, o.p, o.ld, o.dtype, stats ? static_cast<float *>(mean.data_ptr()) : nullptr,
                          stats ? static_cast<float *>(rstd.data_ptr()) : nullptr, fits(T, "x"), fits(d, "x"), on.stream));
+    if (out) written(y);
     if (!stats) return py::cast(y);
     return py::make_tuple(y, mean, rstd);
 }
@@ -263,6 +272,7 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor &dy, c
     check(lib.layer_norm_backward(g.p, g.ld, g.dtype, in.p, in.ld, in.dtype, gm, m, r, o.p, o.ld,
                                   dgamma ? static_cast<float *>(dgamma->data_ptr()) : nullptr, dbeta ? static_cast<float *>(dbeta->data_ptr()) : nullptr,
                                   (int32_t)T, (int32_t)d, ws.data_ptr(), bytes, on.stream));
+    if (out) written(dx);
     return {dx, dgamma, dbeta};
 }
 
@@ -291,6 +301,9 @@ struct GradList {
         list(out, to);
     }
     const omoe_tensor *target() const { return in_place ? nullptr : to.data(); }
+    void scaled() const {
+        for (const Tensor &t : in_place ? grads : out) written(t);
+    }
     Tensor workspace() const { return fresh({OMOE_GRAD_WORKSPACE_BYTES}, at::kByte, device); }
 
     Tensor norm() const {
@@ -303,12 +316,14 @@ struct GradList {
         const auto *p = vec<float>(n, 1, "norm", device);
         const On on(device);
         check(lib.grad_scale(in.data(), target(), (int32_t)in.size(), p, (float)max_norm, on.stream));
+        scaled();
     }
     Tensor clip(double max_norm) const {
         const On on(device);
         const Tensor n = floats({}, device), ws = workspace();
         check(lib.grad_clip(in.data(), target(), (int32_t)in.size(), (float)max_norm, static_cast<float *>(n.data_ptr()), ws.data_ptr(),
                             OMOE_GRAD_WORKSPACE_BYTES, on.stream));
+        scaled();
         return n;
     }
 };
