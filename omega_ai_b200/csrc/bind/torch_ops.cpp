@@ -301,24 +301,36 @@ struct GradList {
         list(out, to);
     }
     const omoe_tensor *target() const { return in_place ? nullptr : to.data(); }
+    // The tensors are still the ones that were checked: theirs is the memory at the addresses kept.
+    void same(bool writes) const {
+        auto moved = [](const std::vector<Tensor> &ts, const std::vector<omoe_tensor> &refs) {
+            bool any = false;
+            for (size_t i = 0; i < ts.size(); i++) any |= ts[i].const_data_ptr() != refs[i].ptr || ts[i].numel() != refs[i].count;
+            return any;
+        };
+        if (moved(grads, in) || (writes && moved(out, to))) bad("a tensor of the list has another storage or size than when the list was built");
+    }
     void scaled() const {
         for (const Tensor &t : in_place ? grads : out) written(t);
     }
     Tensor workspace() const { return fresh({OMOE_GRAD_WORKSPACE_BYTES}, at::kByte, device); }
 
     Tensor norm() const {
+        same(false);
         const On on(device);
         const Tensor n = floats({}, device), ws = workspace();
         check(lib.grad_norm(in.data(), (int32_t)in.size(), static_cast<float *>(n.data_ptr()), ws.data_ptr(), OMOE_GRAD_WORKSPACE_BYTES, on.stream));
         return n;
     }
     void scale(const Tensor &n, double max_norm) const {
+        same(true);
         const auto *p = vec<float>(n, 1, "norm", device);
         const On on(device);
         check(lib.grad_scale(in.data(), target(), (int32_t)in.size(), p, (float)max_norm, on.stream));
         scaled();
     }
     Tensor clip(double max_norm) const {
+        same(true);
         const On on(device);
         const Tensor n = floats({}, device), ws = workspace();
         check(lib.grad_clip(in.data(), target(), (int32_t)in.size(), (float)max_norm, static_cast<float *>(n.data_ptr()), ws.data_ptr(),

@@ -112,8 +112,8 @@ class LNLayer(Layer):
 
 class GradList(_b.GradList):
     """Gradient tensors whose global norm is taken and that are clipped by it: contiguous, fp32 or bf16, on one device,
-    not overlapping.  Built once per set of tensors, which it keeps and whose storage has to stay where it is.  ``out`` (a list of the same sizes and types)
-    receives the clipped gradients; without it they are scaled in place."""
+    not overlapping.  Built once per set of tensors, which it keeps; a call after one of them was resized or given another storage is
+    refused.  ``out`` (a list of the same sizes and types) receives the clipped gradients; without it they are scaled in place."""
 
     def __init__(self, grads, out=None):
         super().__init__(list(grads), None if out is None else list(out))
