@@ -403,7 +403,8 @@ OMOE_API int omoe_unsort_rows_backward(const omoe_sort *plan, const void *dy_dev
  * Layer norm of T rows of width d: y = (x - mean) * rstd * gamma + beta, mean and rstd = 1/sqrt(var + eps) per
  * row, var the mean of the squared differences (taken after the mean, in fp32).  The norm in front of the layer for blocks
  * that are not built on the RMSNorm of omoe_forward_block.  gamma and beta are fp32 [d]; NULL stands for 1 and 0.
- * mean and rstd [T] fp32 are written unless NULL; the backward pass takes them.  T <= 0x7fff0000.
+ * mean and rstd [T] fp32 are written unless NULL; the backward pass takes them.  T <= 0x7fff0000.  Rows move as vectors
+ * only where gamma and beta (forward) or gamma (backward) are NULL or aligned to 8 elements too: 32 bytes.
  *
  * omoe_layer_norm_backward: with g = dy * gamma and h = (x - mean) * rstd,
  *   dx = rstd * (g - mean(g) - h * mean(g * h)) of x's element type, dgamma = sum over the rows of dy * h,

@@ -915,6 +915,8 @@ int omoe_layer_norm(const void *x_dev, int64_t ldx, int32_t x_dtype, const float
         using XT = std::remove_pointer_t<decltype(xt)>;
         using YT = std::remove_pointer_t<decltype(yt)>;
         cudaError_t e = cudaSuccess;
+        // (parameters that may lie anywhere, behind a branch in the kernels, cost the aligned ones: 65536 x 1024 of bf16 44 -> 45 us, 4096 x 16384
+        // 58 -> 66 and backward 113 -> 138)
         const bool vec = rows_vector(x) && rows_vector(y) && !misaligned(gamma_dev, 32) && !misaligned(beta_dev, 32);
         if (by_width<false, XT, YT>(vec, T, d,
                      [&](auto v, auto g, auto p) {

@@ -72,8 +72,9 @@ class TokenSort(_b.TokenSort):
 
 
 def layer_norm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=None, dtype=None, stats: bool = False):
-    """(x - mean) * rstd * gamma + beta per row of x [T, d]; gamma and beta [d] fp32, None for 1 and 0.  With ``stats``
-    (y, mean, rstd), which :func:`layer_norm_backward` takes."""
+    """(x - mean) * rstd * gamma + beta per row of x [T, d]; gamma and beta [d] fp32, None for 1 and 0; at addresses
+    that are not multiples of 32 bytes they send the rows through the slower kernels for single elements.  With ``stats`` (y, mean, rstd), which
+    :func:`layer_norm_backward` takes."""
     return _b.layer_norm(x, gamma, beta, eps, out, dtype, stats)
 
 

@@ -7,7 +7,7 @@ x - mean carries one rounding and h two: with H = |h| (1 + 2 u)
   dgamma      (T / 8 + 80) u of the sum over the rows of |dy| H."""
 import pytest
 import torch
-from test_layer_norm_gpu import BF, F32, HALF, U, rows
+from test_layer_norm_gpu import BF, F32, HALF, U, forward_bounds, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,39 @@ def test_means_of_infinite_sums():
         x[0, d // 2], x[1, 0], x[2, 1], x[2, d - 1], x[3, 3] = float("inf"), -float("inf"), float("inf"), -float("inf"), float("nan")
         _, mean, _ = layer_norm(x, stats=True)
         assert mean[0] == float("inf") and mean[1] == -float("inf") and mean[2:].isnan().all()
+
+
+@pytest.mark.parametrize("xt,yt", [(BF, BF), (F32, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("d", [8, 264, 520, 776, 1024, 2224, 4096, 5120, 8192, 9000, 16384, 20000])
+def test_parameters_at_any_address(d, xt, yt):
+    """Aligned rows with gamma and beta at odd elements of a buffer, or at 16 bytes, which go another way than with aligned parameters."""
+    from omega_ai_b200 import layer_norm, layer_norm_backward
+
+    T = 40
+    x, _ = rows(T, d, xt, "packed", 1)
+    dy, _ = rows(T, d, yt, "packed", 2)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    gamma, beta = torch.randn(d, generator=gen, device="cuda"), torch.randn(d, generator=gen, device="cuda")
+    D = d / 32 + 40
+    for a, b in ((1, 0), (0, 1), (4, 4), (3, 2), (8, 5)):
+        flat = torch.full((2 * d + 64,), float("nan"), device="cuda")  # what lies beside the parameters is not used
+        g, s = flat[a:a + d], flat[d + 32 + b:][:d]
+        g.copy_(gamma)
+        s.copy_(beta)
+        y, mean, rstd = layer_norm(x, g, s, dtype=yt, stats=True)
+        m, m_off, r, r_off, ref, off = forward_bounds(x, gamma, beta, 1e-5, yt)
+        assert ((mean.double() - m[:, 0]).abs() <= m_off[:, 0] * 1.01 + U * m[:, 0].abs()).all()
+        assert ((rstd.double() - r[:, 0]).abs() <= r_off[:, 0]).all()
+        assert ((y.double() - ref).abs() <= off).all()
+        dx, dgamma, dbeta = layer_norm_backward(dy, x, g, mean, rstd)
+        m, r = mean.double().unsqueeze(1), rstd.double().unsqueeze(1)
+        gr, h = dy.double() * gamma.double(), (x.double() - m) * r
+        H = h.abs() + r * U * m.abs()
+        mg, mh = gr.mean(1, keepdim=True), (gr * h).mean(1, keepdim=True)
+        mg_off, mh_off = ((D + 4) * U * t.abs().mean(1, keepdim=True) for t in (gr, gr.abs() * H))
+        ref = r * (gr - mg - h * mh)
+        off = r * (mg_off + H * mh_off + 8 * U * (gr.abs() + mg.abs() + H * mh.abs()))
+        assert ((dx.double() - ref).abs() <= off * 1.01 + HALF[xt] * (ref.abs() + off)).all()
+        n = (T / 8 + 80) * U
+        assert ((dgamma.double() - (dy.double() * h).sum(0)).abs() <= n * (dy.double().abs() * H).sum(0)).all()
+        assert ((dbeta.double() - dy.double().sum(0)).abs() <= n * dy.double().abs().sum(0)).all()
