@@ -134,12 +134,14 @@ void written(const Tensor &t) {
 Tensor matrix_or_new(const OptTensor &out, int64_t rows, int64_t d, at::ScalarType type, const c10::Device &device) {
     return out ? *out : fresh({rows, d}, type, device);
 }
-// A vector of n floats and a second one behind it in the same storage: what lives and dies together takes one allocation.
+// A vector of n floats and a second one behind it in the same storage: what lives and dies together takes one allocation.  The second starts on a
+// vector of its own, so that both move as vectors where they go next (a list of gradients).
 std::pair<Tensor, Tensor> two_floats(int64_t n, const c10::Device &device) {
-    Tensor a = fresh({2 * n}, at::kFloat, device);
+    const int64_t second = (n + 7) / 8 * 8;
+    Tensor a = fresh({second + n}, at::kFloat, device);
     auto b = c10::make_intrusive<c10::TensorImpl>(c10::Storage(a.storage()), a.key_set(), a.dtype());
     b->set_sizes_contiguous({n});
-    b->set_storage_offset(n);
+    b->set_storage_offset(second);
     a.unsafeGetTensorImpl()->set_sizes_contiguous({n});
     return {a, Tensor(std::move(b))};
 }

@@ -80,7 +80,8 @@ def layer_norm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=No
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma, mean: torch.Tensor, rstd: torch.Tensor, out=None,
                         param_grads: bool = True):
-    """(dx, dgamma, dbeta) of :func:`layer_norm`; without ``param_grads`` the last two are None."""
+    """(dx, dgamma, dbeta) of :func:`layer_norm`; without ``param_grads`` the last two are None.  dgamma and dbeta share a storage, as
+    mean and rstd do."""
     return _b.layer_norm_backward(dy, x, gamma, mean, rstd, out, param_grads)
 
 

@@ -119,3 +119,21 @@ def test_parameters_at_any_address(d, xt, yt):
         n = (T / 8 + 80) * U
         assert ((dgamma.double() - (dy.double() * h).sum(0)).abs() <= n * (dy.double().abs() * H).sum(0)).all()
         assert ((dbeta.double() - dy.double().sum(0)).abs() <= n * dy.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("T,d", [(1, 1), (3, 7), (5, 1001), (8, 1024)])
+def test_gradients_and_statistics_are_aligned(T, d):
+    """dgamma and dbeta, mean and rstd lie side by side, apart and each on a vector of its own, whatever the sizes."""
+    from omega_ai_b200 import GradList, layer_norm, layer_norm_backward
+
+    x = torch.randn(T, d, device="cuda")
+    _, mean, rstd = layer_norm(x, stats=True)
+    _, dgamma, dbeta = layer_norm_backward(x, x, None, mean, rstd)
+    assert all(t.data_ptr() % 32 == 0 and t.is_contiguous() for t in (mean, rstd, dgamma, dbeta))
+    assert mean.shape == rstd.shape == (T,) and dgamma.shape == dbeta.shape == (d,)
+    want, beta = dgamma.clone(), dbeta.clone()
+    GradList([dbeta]).clip(0.0)
+    assert torch.equal(dgamma, want) and (dbeta == 0).all()
+    dbeta.copy_(beta)
+    dgamma.zero_()
+    assert torch.equal(dbeta, beta)
