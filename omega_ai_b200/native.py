@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import warnings
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 # OMOE_LIB selects another build of the same ABI, e.g. the self-checking one (libomoe_check.so, csrc/check.cu)
@@ -87,13 +88,17 @@ def sources():
 
 def build(force: bool = False, check: bool = False) -> str:
     """Compile ``libomoe.so`` for sm_100a with nvcc (cross-compiles without a GPU); with ``check`` the
-    self-checking variant ``libomoe_check.so`` (-DOMOE_BOUNDS_CHECK)."""
+    self-checking variant ``libomoe_check.so`` (-DOMOE_BOUNDS_CHECK).  The operators' torch binding is built beside ``libomoe.so``; where
+    torch or a C++ compiler is missing that is a warning, for hosts that use the library alone."""
     path = CHECK_LIB_PATH if check else os.path.join(_PKG, "libomoe.so")
     stale = (not os.path.exists(path)) or any(os.path.getmtime(s) > os.path.getmtime(path) for s in sources())
     if force or stale:
         subprocess.check_call(["sh", os.path.join(CSRC, "build.sh")] + (["check"] if check else []))
     if not check:
-        build_binding(force)
+        try:
+            build_binding(force)
+        except (ImportError, OSError, subprocess.CalledProcessError) as e:
+            warnings.warn(f"_torch_ops.so is not built ({e}): omega_ai_b200.ops needs it, libomoe.so does not", stacklevel=2)
     return path
 
 
