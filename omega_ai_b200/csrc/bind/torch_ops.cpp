@@ -16,6 +16,9 @@
 
 #include "../../../include/omoe.h"
 
+// The torch and the Python that this is built for; native.build_binding() looks for it in the file.
+extern "C" __attribute__((visibility("default"), used)) const char omoe_binding_mark[] = OMOE_BINDING_MARK;
+
 namespace py = pybind11;
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;

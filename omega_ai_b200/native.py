@@ -102,19 +102,37 @@ def build(force: bool = False, check: bool = False) -> str:
     return path
 
 
+def binding_mark() -> str:
+    """What a binding for the installed torch and Python carries: their interfaces differ from version to version."""
+    import sysconfig
+
+    import torch
+
+    return f"omoe torch_ops for torch {torch.__version__} {sysconfig.get_config_var('SOABI')}."
+
+
 def build_binding(force: bool = False) -> str:
-    """Compile ``_torch_ops.so``, the operators' binding for torch tensors, against the installed torch."""
+    """Compile ``_torch_ops.so``, the operators' binding for torch tensors, against the installed torch, where it is older than its
+    sources or was built for another torch or Python."""
     import sysconfig
 
     import torch
 
     src, header = os.path.join(CSRC, "bind", "torch_ops.cpp"), os.path.join(os.path.dirname(_PKG), "include", "omoe.h")
     path = os.path.join(_PKG, "_torch_ops.so")
-    if force or not os.path.exists(path) or any(os.path.getmtime(s) > os.path.getmtime(path) for s in (src, header)):
+    mark = binding_mark()
+
+    def fresh():
+        if not os.path.exists(path) or any(os.path.getmtime(s) > os.path.getmtime(path) for s in (src, header)):
+            return False
+        with open(path, "rb") as f:
+            return mark.encode() in f.read()
+
+    if force or not fresh():
         home, cuda = os.path.dirname(torch.__file__), os.environ.get("CUDA_HOME", "/usr/local/cuda")
         subprocess.check_call(
             [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
+             f'-DOMOE_BINDING_MARK="{mark}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
              f"-I{home}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", src,
              "-o", path, f"-L{home}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"])
     return path

@@ -23,7 +23,7 @@ def _bind():
     try:
         from . import _torch_ops
     except ImportError as e:
-        raise ImportError(f"omega_ai_b200/_torch_ops.so cannot be loaded ({e}): build it with omega_ai_b200.native.build()") from e
+        raise ImportError(f"omega_ai_b200/_torch_ops.so cannot be loaded ({e}): build it with omega_ai_b200.native.build_binding()") from e
     L = native.lib()
     _torch_ops.init({n: C.cast(getattr(L, n), C.c_void_p).value for n in native.OPERATORS}, OmoeError)
     return _torch_ops

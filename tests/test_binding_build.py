@@ -25,3 +25,55 @@ def test_the_library_is_built_where_the_binding_cannot_be(monkeypatch):
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         native.build()
+
+
+@pytest.fixture
+def package(tmp_path, monkeypatch):
+    """A package folder of its own with a stand-in for the compiler: `write` is what it leaves at its -o, `status` its exit status."""
+    pkg = tmp_path / "omega_ai_b200"
+    pkg.mkdir()
+    shutil.copytree(os.path.join(ROOT, "include"), tmp_path / "include")
+    monkeypatch.setattr(native, "_PKG", str(pkg))
+
+    def compiler(write, status=0):
+        cxx = tmp_path / "cxx"
+        cxx.write_text('#!/bin/sh\nfor a in "$@"; do echo "$a" >> %s/args; done\nwhile [ "$1" != -o ]; do shift; done\nprintf %%s "%s" > "$2"\nexit %d\n'
+                       % (tmp_path, write, status))
+        cxx.chmod(cxx.stat().st_mode | stat.S_IXUSR)
+        monkeypatch.setenv("CXX", str(cxx))
+
+    return pkg, compiler
+
+
+def later(path):
+    """Newer than any source."""
+    at = max(os.path.getmtime(os.path.join(native.CSRC, "bind", "torch_ops.cpp")), path.stat().st_mtime) + 100
+    os.utime(path, (at, at))
+
+
+def test_a_binding_for_another_torch_is_built_again(package):
+    import torch
+
+    pkg, compiler = package
+    so = pkg / "_torch_ops.so"
+    so.write_text("built for another torch")
+    later(so)
+    compiler("new")
+    assert native.build_binding() == str(so)
+    assert so.read_text() == "new"
+    # one for the installed torch and Python stays: the compiler is given the mark that it has to carry
+    given = [a for a in (pkg.parent / "args").read_text().splitlines() if torch.__version__ in a]
+    assert len(given) == 1
+    so.write_text("code " + given[0].split("=", 1)[1].strip('"') + " code")
+    later(so)
+    compiler("newer")
+    native.build_binding()
+    assert so.read_text() != "newer"
+
+
+def test_the_built_binding_carries_its_mark():
+    native.build()
+    path = native.build_binding()
+    before = os.stat(path).st_mtime_ns
+    assert native.build_binding() == path and os.stat(path).st_mtime_ns == before
+    assert native.binding_mark().encode() in open(path, "rb").read()
