@@ -130,11 +130,17 @@ def build_binding(force: bool = False) -> str:
 
     if force or not fresh():
         home, cuda = os.path.dirname(torch.__file__), os.environ.get("CUDA_HOME", "/usr/local/cuda")
-        subprocess.check_call(
-            [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-             f'-DOMOE_BINDING_MARK="{mark}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
-             f"-I{home}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", src,
-             "-o", path, f"-L{home}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"])
+        made = os.path.join(_PKG, f"_torch_ops.{os.getpid()}.so")  # whole before it gets its name: other processes may be loading or building it
+        try:
+            subprocess.check_call(
+                [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                 f'-DOMOE_BINDING_MARK="{mark}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
+                 f"-I{home}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", src,
+                 "-o", made, f"-L{home}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"])
+            os.replace(made, path)
+        finally:
+            if os.path.exists(made):
+                os.remove(made)
     return path
 
 

@@ -77,3 +77,19 @@ def test_the_built_binding_carries_its_mark():
     before = os.stat(path).st_mtime_ns
     assert native.build_binding() == path and os.stat(path).st_mtime_ns == before
     assert native.binding_mark().encode() in open(path, "rb").read()
+
+
+def test_a_build_that_fails_leaves_the_binding_alone(package):
+    """The file appears whole or not at all: a process that loads it meanwhile, or after a failed build, does not find half of one."""
+    pkg, compiler = package
+    so = pkg / "_torch_ops.so"
+    so.write_text("whole")
+    compiler("half", status=1)
+    with pytest.raises(subprocess.CalledProcessError):
+        native.build_binding(force=True)
+    assert so.read_text() == "whole" and [p.name for p in pkg.iterdir()] == ["_torch_ops.so"]
+    compiler("next")
+    with open(so) as held:  # as a process that has it loaded
+        native.build_binding(force=True)
+        assert held.read() == "whole" and so.read_text() == "next"
+    assert [p.name for p in pkg.iterdir()] == ["_torch_ops.so"]
