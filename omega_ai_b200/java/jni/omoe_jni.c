@@ -161,49 +161,47 @@ JFN(jlong, sortRowsCap)(JNIEnv *env, jclass c, jint T, jint k, jint E, jint alig
     return omoe_sort_rows_cap(T, k, E, align);
 }
 
-/* The plan's sizes and addresses, 9 longs; false where there are fewer or a size does not fit. */
-static int read_plan(JNIEnv *env, jlongArray plan, omoe_sort *p) {
-    if (!plan || (*env)->GetArrayLength(env, plan) < 9) return 0;
+/* The plan's sizes and addresses, 9 longs; NULL, which the library refuses, where there are fewer or a size does not fit. */
+static const omoe_sort *read_plan(JNIEnv *env, jlongArray plan, omoe_sort *p) {
+    if (!plan || (*env)->GetArrayLength(env, plan) < 9) return NULL;
     jlong *v = (*env)->GetLongArrayElements(env, plan, NULL);
-    if (!v) return 0;
+    if (!v) return NULL;
     int ok = 1;
     for (int i = 0; i < 4; i++) ok = ok && v[i] >= INT32_MIN && v[i] <= INT32_MAX;
     p->n_tokens = (int32_t)v[0]; p->top_k = (int32_t)v[1]; p->n_experts = (int32_t)v[2]; p->row_align = (int32_t)v[3];
     p->rows_cap = v[4];
     p->pos = (int32_t *)P(v[5]); p->perm = (int32_t *)P(v[6]); p->counts = (int32_t *)P(v[7]); p->offsets = (int32_t *)P(v[8]);
     (*env)->ReleaseLongArrayElements(env, plan, v, JNI_ABORT);
-    return ok;
+    return ok ? p : NULL;
 }
 
 JFN(jint, sortPlan)(JNIEnv *env, jclass c, jlongArray plan, jlong idx) {
     omoe_sort p;
-    return read_plan(env, plan, &p) ? omoe_sort_plan(&p, (const int32_t *)P(idx), NULL) : OMOE_ERR_INVALID;
+    return omoe_sort_plan(read_plan(env, plan, &p), (const int32_t *)P(idx), NULL);
 }
 
 JFN(jint, sortRows)(JNIEnv *env, jclass c, jlongArray plan, jlong x, jlong ldx, jint xdt, jlong xs, jlong ldxs, jint xsdt, jint d) {
     omoe_sort p;
-    return read_plan(env, plan, &p) ? omoe_sort_rows(&p, P(x), ldx, xdt, P(xs), ldxs, xsdt, d, NULL) : OMOE_ERR_INVALID;
+    return omoe_sort_rows(read_plan(env, plan, &p), P(x), ldx, xdt, P(xs), ldxs, xsdt, d, NULL);
 }
 
 JFN(jint, sortRowsBackward)(JNIEnv *env, jclass c, jlongArray plan, jlong dxs, jlong lddxs, jint dxsdt, jlong dx, jlong lddx,
                             jint dxdt, jint d) {
     omoe_sort p;
-    return read_plan(env, plan, &p) ? omoe_sort_rows_backward(&p, P(dxs), lddxs, dxsdt, P(dx), lddx, dxdt, d, NULL) : OMOE_ERR_INVALID;
+    return omoe_sort_rows_backward(read_plan(env, plan, &p), P(dxs), lddxs, dxsdt, P(dx), lddx, dxdt, d, NULL);
 }
 
 JFN(jint, unsortRows)(JNIEnv *env, jclass c, jlongArray plan, jlong ys, jlong ldys, jint ysdt, jlong w, jlong y, jlong ldy,
                       jint ydt, jint d) {
     omoe_sort p;
-    return read_plan(env, plan, &p) ? omoe_unsort_rows(&p, P(ys), ldys, ysdt, (const float *)P(w), P(y), ldy, ydt, d, NULL)
-                                    : OMOE_ERR_INVALID;
+    return omoe_unsort_rows(read_plan(env, plan, &p), P(ys), ldys, ysdt, (const float *)P(w), P(y), ldy, ydt, d, NULL);
 }
 
 JFN(jint, unsortRowsBackward)(JNIEnv *env, jclass c, jlongArray plan, jlong dy, jlong lddy, jint dydt, jlong ys, jlong ldys,
                               jint ysdt, jlong w, jlong dys, jlong lddys, jlong dw, jint d) {
     omoe_sort p;
-    return read_plan(env, plan, &p) ? omoe_unsort_rows_backward(&p, P(dy), lddy, dydt, P(ys), ldys, ysdt, (const float *)P(w),
-                                                                P(dys), lddys, (float *)P(dw), d, NULL)
-                                    : OMOE_ERR_INVALID;
+    return omoe_unsort_rows_backward(read_plan(env, plan, &p), P(dy), lddy, dydt, P(ys), ldys, ysdt, (const float *)P(w),
+                                     P(dys), lddys, (float *)P(dw), d, NULL);
 }
 
 JFN(jint, layerNorm)(JNIEnv *env, jclass c, jlong x, jlong ldx, jint xdt, jlong gamma, jlong beta, jfloat eps, jlong y, jlong ldy,
@@ -222,7 +220,7 @@ JFN(jint, layerNormBackward)(JNIEnv *env, jclass c, jlong dy, jlong lddy, jint d
                                     wsBytes, NULL);
 }
 
-/* Host table of the tensors, to be freed; *n is -1 where the arrays do not agree or memory is short. */
+/* Host table of the tensors, to be freed; *n is -1, which the library refuses, where the arrays do not agree or memory is short. */
 static omoe_tensor *read_tensors(JNIEnv *env, jlongArray ptrs, jlongArray counts, jintArray dtypes, jint *n) {
     *n = -1;
     if (!ptrs || !counts || !dtypes) return NULL;
@@ -247,7 +245,7 @@ static omoe_tensor *read_tensors(JNIEnv *env, jlongArray ptrs, jlongArray counts
 JFN(jint, gradNorm)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray dt, jlong norm, jlong ws, jlong wsBytes) {
     jint m;
     omoe_tensor *t = read_tensors(env, g, n, dt, &m);
-    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_norm(t, m, (float *)P(norm), P(ws), wsBytes, NULL);
+    int rc = omoe_grad_norm(t, m, (float *)P(norm), P(ws), wsBytes, NULL);
     free(t);
     return rc;
 }
@@ -255,7 +253,7 @@ JFN(jint, gradNorm)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray
 JFN(jint, gradScale)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray dt, jlong norm, jfloat maxNorm) {
     jint m;
     omoe_tensor *t = read_tensors(env, g, n, dt, &m);
-    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_scale(t, NULL, m, (const float *)P(norm), maxNorm, NULL);
+    int rc = omoe_grad_scale(t, NULL, m, (const float *)P(norm), maxNorm, NULL);
     free(t);
     return rc;
 }
@@ -264,7 +262,7 @@ JFN(jint, gradClip)(JNIEnv *env, jclass c, jlongArray g, jlongArray n, jintArray
                     jlong wsBytes) {
     jint m;
     omoe_tensor *t = read_tensors(env, g, n, dt, &m);
-    int rc = m < 0 ? OMOE_ERR_INVALID : omoe_grad_clip(t, NULL, m, maxNorm, (float *)P(norm), P(ws), wsBytes, NULL);
+    int rc = omoe_grad_clip(t, NULL, m, maxNorm, (float *)P(norm), P(ws), wsBytes, NULL);
     free(t);
     return rc;
 }
