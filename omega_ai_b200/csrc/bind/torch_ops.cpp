@@ -150,6 +150,11 @@ std::pair<Tensor, Tensor> two_floats(int64_t n, const c10::Device &device) {
 }
 Tensor floats(at::IntArrayRef sizes, const c10::Device &device) { return fresh(sizes, at::kFloat, device); }
 
+// A call's dtype is for the tensor that it makes: beside `out` it may only repeat that one's.
+void agree(const OptTensor &out, const std::optional<at::ScalarType> &dtype) {
+    if (out && dtype && out->scalar_type() != *dtype) bad(std::string("dtype: out has ") + c10::toString(out->scalar_type()) + ", not " + c10::toString(*dtype));
+}
+
 int64_t width(const Tensor &t, const char *name) {
     if (t.dim() != 2) bad(std::string(name) + ": expected a matrix, got " + text(t.sizes()));
     return t.size(1);
@@ -180,16 +185,24 @@ struct TokenSort {
         return {(int32_t)tokens, (int32_t)top_k, (int32_t)n_experts, (int32_t)row_align, rows_cap, static_cast<int32_t *>(pos.data_ptr()),
                 static_cast<int32_t *>(perm.data_ptr()), static_cast<int32_t *>(counts.data_ptr()), static_cast<int32_t *>(offsets.data_ptr())};
     }
-    const float *weights_of(const OptTensor &w) const { return vec<float>(w, tokens * top_k, "weights", device); }
+    // One value for every pick: [tokens, top_k], or without a shape.
+    template <typename T>
+    T *of_picks(const OptTensor &t, const char *name, at::ScalarType type) const {
+        if (t && t->dim() == 2 && (t->size(0) != tokens || t->size(1) != top_k))
+            bad(std::string(name) + ": expected " + text({tokens, top_k}) + ", got " + text(t->sizes()));
+        return vec<T>(t, tokens * top_k, name, device, type);
+    }
+    const float *weights_of(const OptTensor &w) const { return of_picks<float>(w, "weights", at::kFloat); }
 
     void plan(const Tensor &topk_idx) const {
-        const auto *idx = vec<int32_t>(topk_idx, tokens * top_k, "topk_idx", device, at::kInt);
+        const auto *idx = of_picks<int32_t>(topk_idx, "topk_idx", at::kInt);
         const On on(device);
         const omoe_sort p = c();
         check(lib.sort_plan(&p, idx, on.stream));
     }
     Tensor sort(const Tensor &x, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
         const int64_t d = width(x, "x");
+        agree(out, dtype);
         const Matrix in(x, tokens, d, "x", device);
         const On on(device);
         Tensor to = matrix_or_new(out, rows_cap, d, dtype.value_or(x.scalar_type()), device);
@@ -201,6 +214,7 @@ struct TokenSort {
     }
     Tensor sort_backward(const Tensor &dxs, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
         const int64_t d = width(dxs, "dxs");
+        agree(out, dtype);
         const Matrix in(dxs, rows_cap, d, "dxs", device);
         const On on(device);
         Tensor to = matrix_or_new(out, tokens, d, dtype.value_or(dxs.scalar_type()), device);
@@ -212,6 +226,7 @@ struct TokenSort {
     }
     Tensor unsort(const Tensor &ys, const OptTensor &weights, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
         const int64_t d = width(ys, "ys");
+        agree(out, dtype);
         const Matrix in(ys, rows_cap, d, "ys", device);
         const float *w = weights_of(weights);
         const On on(device);
@@ -246,6 +261,7 @@ py::object layer_norm(const Tensor &x, const OptTensor &gamma, const OptTensor &
                       const std::optional<at::ScalarType> &dtype, bool stats) {
     const int64_t d = width(x, "x"), T = x.size(0);
     const c10::Device dev = x.device();
+    agree(out, dtype);
     const Matrix in(x, T, d, "x", dev);
     const auto *g = vec<float>(gamma, d, "gamma", dev), *b = vec<float>(beta, d, "beta", dev);
     const On on(dev);
