@@ -8,6 +8,8 @@
 #include <math.h>
 #include <stdlib.h>
 
+#include <algorithm>
+
 namespace omoe {
 
 namespace {
@@ -230,10 +232,6 @@ struct Span {
     uintptr_t lo, hi;
     int32_t i;
 };
-int by_address(const void *a, const void *b) {
-    const Span *x = static_cast<const Span *>(a), *y = static_cast<const Span *>(b);
-    return x->lo < y->lo ? -1 : x->lo > y->lo;
-}
 
 // The spans of a list by address, empty tensors left out; returns how many.
 int spans_of(const omoe_tensor *t, int n, Span *s) {
@@ -247,7 +245,7 @@ int spans_of(const omoe_tensor *t, int n, Span *s) {
         sorted = sorted && (m == 0 || s[m - 1].lo <= s[m].lo);
         m++;
     }
-    if (!sorted) qsort(s, m, sizeof(Span), by_address);
+    if (!sorted) std::sort(s, s + m, [](const Span &a, const Span &b) { return a.lo < b.lo; });
     return m;
 }
 
