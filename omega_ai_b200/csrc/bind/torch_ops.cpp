@@ -1,8 +1,8 @@
 // Binding of the operators without a handle (include/omoe.h) for torch tensors.
 //
 // A call of these operators on a small batch is mostly its way to the GPU: through ctypes, with the checks of the tensors and the
-// allocations made in Python, 7 to 12 us of the host against 2 to 6 on the device.  Here the same checks, allocations and
-// the call itself take about 4.  The entry points are not linked: init() gets their addresses from the library
+// allocations made in Python, 7 to 19 us of the host against 2 to 10 on the device.  Here the same checks, allocations and
+// the call itself take 2.5 to 7.  The entry points are not linked: init() gets their addresses from the library
 // that native.py has loaded, so that there is one copy of it in the process.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>

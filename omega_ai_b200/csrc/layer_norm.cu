@@ -207,7 +207,6 @@ __device__ __forceinline__ f2 pack2(float a, float b) {
     return r;
 }
 __device__ __forceinline__ void unpack2(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-// (the result is a register pair of its own: tied to an operand that is needed again, each would cost two moves)
 __device__ __forceinline__ f2 add2(f2 a, f2 b) {
     f2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
