@@ -130,7 +130,7 @@ T *vec(const OptTensor &t, int64_t n, const char *name, const c10::Device &devic
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const c10::Device &device) {
     return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
-// A caller's tensor was written: autograd has to refuse what saved it before.
+// A tensor that the caller has was written: autograd has to refuse what saved it before.
 void written(const Tensor &t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -199,6 +199,7 @@ struct TokenSort {
         const On on(device);
         const omoe_sort p = c();
         check(lib.sort_plan(&p, idx, on.stream));
+        for (const Tensor *t : {&pos, &perm, &counts, &offsets}) written(*t);
     }
     Tensor sort(const Tensor &x, const OptTensor &out, const std::optional<at::ScalarType> &dtype) const {
         const int64_t d = width(x, "x");

@@ -5,7 +5,7 @@ Calls enqueue on the current stream of the tensors' device and do not synchronis
 that may lie apart (``stride(0) >= d``, ``stride(1) == 1``), fp32 or bf16.  What a call needs besides its arguments it
 takes from the caching allocator, so calls on different streams and captured graphs share nothing.  Autograd records none of them: results are detached, also from
 inputs that require gradients, and the backward passes are calls of their own.  What a call writes of its caller's (``out``, gradients
-clipped in place) counts as modified in place.  Tensors are checked and
+clipped in place, a plan's tensors) counts as modified in place.  Tensors are checked and
 the library is called in ``_torch_ops.so`` (csrc/bind/torch_ops.cpp): a small batch is over before Python has looked at its tensors.
 """
 from __future__ import annotations

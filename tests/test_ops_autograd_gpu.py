@@ -63,3 +63,19 @@ def test_read_tensors_stay_as_they_were():
     GradList([x]).norm()
     GradList([x], out=[torch.empty_like(x)]).clip(0.5)
     assert x._version == version
+
+
+def test_a_new_plan_is_known_to_autograd():
+    """Rows gathered by a plan's perm have a gradient by that perm: not by the next plan's."""
+    from omega_ai_b200 import TokenSort
+
+    sort = TokenSort(6, 2, 4)
+    idx = torch.randint(0, 4, (6, 2), dtype=torch.int32, device="cuda")
+    before = [t._version for t in (sort.pos, sort.perm, sort.counts, sort.offsets)]
+    sort.plan(idx)
+    assert all(t._version > v for t, v in zip((sort.pos, sort.perm, sort.counts, sort.offsets), before))
+    picks = torch.randn(12, 8, device="cuda", requires_grad=True)
+    y = picks.index_select(0, sort.perm).sum()  # saves perm
+    sort.plan(idx.flip(0).contiguous())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
